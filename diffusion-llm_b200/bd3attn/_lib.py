@@ -59,6 +59,13 @@ SIGNATURES = {
                                _vp]),
     "bd3_subs_sample_dev": (_i32, [_vp, _pi64, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _i32,
                                    _vp]),
+    "bd3_paged_workspace_size": (_sz, []),
+    "bd3_paged_attn": (_i32, [_vp] * 8 + [_i64] * 9 + [_pi64, _i64, ctypes.c_double, _i32, _i32,
+                                                       _vp, _sz, _vp]),
+    "bd3_qkv_rope_paged": (_i32, [_vp] + [_i64] * 6 + [_vp, _vp, _i64] + [_vp] * 6 + [_i64] * 3 +
+                           [_pi64, _i32, _vp]),
+    "bd3_process_logits": (_i32, [_vp, _vp, _pi64, _i64, _i64, _i64, _vp, _i32, _i64, _i64] +
+                           [_vp] * 5 + [_i64, _vp, _pi64, _i32, _vp]),
     "bd3_profile_enable": (_i32, [_i32]),
     "bd3_profile_collect": (_i32, [ctypes.POINTER(ctypes.c_double), _pi32]),
     "bd3_debug_ranges": (_i32, [_i32, _i64, _i64, _i64, _i64, _i64, _i64, _pi32]),

@@ -376,6 +376,160 @@ def _(qkv, n_heads, cos_table, sin_table, k_cache, v_cache, row0, positions=None
 
 
 # ---------------------------------------------------------------------------------------
+# Paged KV cache
+def _on_device(device, fn, *args):
+    """fn(*args) with `device` current (the context manager only where it changes something)."""
+    if torch.cuda.current_device() == device.index:
+        return fn(*args)
+    with torch.cuda.device(device):
+        return fn(*args)
+
+
+def _check_pages(k_pages, v_pages, page_table, kv_lens, cu_q, dtype, n_kv_heads, D):
+    _check_cuda(k_pages, v_pages, page_table, kv_lens, cu_q)
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.shape[1] != n_kv_heads \
+            or k_pages.shape[3] != D:
+        raise AssertionError("k_pages and v_pages must be (pages, kv heads, page size, head_dim)")
+    if k_pages.dtype != dtype or v_pages.dtype != dtype:
+        raise AssertionError("k_pages and v_pages must be in the new tokens' dtype")
+    if k_pages.stride(3) != 1 or v_pages.stride(3) != 1:
+        raise AssertionError("the pages' head_dim must be contiguous")
+    if page_table.dtype != torch.int32 or kv_lens.dtype != torch.int32 \
+            or cu_q.dtype != torch.int32:
+        raise AssertionError("page_table, kv_lens and cu_q must be int32")
+    B = kv_lens.shape[0]
+    if page_table.dim() != 2 or page_table.shape[0] != B or page_table.stride(1) != 1 \
+            or cu_q.shape != (B + 1,) or kv_lens.dim() != 1 or not cu_q.is_contiguous() \
+            or not kv_lens.is_contiguous():
+        raise AssertionError("page_table must be (B, pages), kv_lens (B,) and cu_q (B + 1,)")
+    return B
+
+
+def paged_workspace(device=None) -> torch.Tensor:
+    """A workspace for paged_attn_raw on `device` (bd3_paged_workspace_size bytes, zeroed). Keep
+    it and pass it to every call; calls that share one must be ordered (one stream)."""
+    device = torch.device("cuda", torch.cuda.current_device()) if device is None \
+        else torch.device(device)
+    with torch.cuda.device(device):
+        n = LIB.bd3_paged_workspace_size()
+        if n == 0:
+            check("bd3_paged_workspace_size", 3)
+        return torch.zeros(n, dtype=torch.uint8, device=device)
+
+
+def paged_attn_raw(q, k_pages, v_pages, page_table, kv_lens, cu_q, max_q_len: int,
+                   block_size: int, scale: float | None = None, out_dtype=None,
+                   return_lse: bool = False, workspace=None):
+    """Block-causal attention of packed new tokens over a paged KV cache.
+
+    q: (tokens, q heads, 64) bf16/f16, sequence b's rows [cu_q[b], cu_q[b+1]); k_pages, v_pages:
+    (pages, kv heads, page size, 64) in q's dtype, any strides, page size a multiple of 8;
+    page_table: (B, pages per sequence) int32; kv_lens: (B,) int32 positions of each sequence,
+    the new tokens (its last ones) included; cu_q: (B + 1,) int32; max_q_len: the most new
+    tokens of a sequence. Tensors of lengths stay on the device: a captured CUDA graph serves
+    other lengths and tables. workspace: paged_workspace(), kept by the caller (None: a new
+    zeroed one). Returns O (tokens, q heads, 64), with the LSE (tokens, q heads) if asked.
+    """
+    _check_cuda(q)
+    if q.dim() != 3:
+        raise AssertionError("q must be (tokens, q heads, head_dim)")
+    T, Hq, D = q.shape
+    Hkv = k_pages.shape[1]
+    B = _check_pages(k_pages, v_pages, page_table, kv_lens, cu_q, q.dtype, Hkv, D)
+    if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
+    code = _code(q.dtype)
+    out_dtype = q.dtype if out_dtype is None else out_dtype
+    dev = q.device
+    o = torch.empty((T, Hq, D), dtype=out_dtype, device=dev)
+    lse = torch.empty((T, Hq), dtype=torch.float32, device=dev) if return_lse else None
+    if workspace is None:
+        workspace = paged_workspace(dev)
+    elif workspace.device != dev:
+        raise AssertionError("the workspace must be on q's device")
+    ks, vs = k_pages.stride(), v_pages.stride()
+    strides = i64_array((q.stride(0), q.stride(1), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
+                         Hq * D, D, page_table.stride(0)))
+    check("bd3_paged_attn", _on_device(
+        dev, LIB.bd3_paged_attn, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+        o.data_ptr(), lse.data_ptr() if return_lse else None, page_table.data_ptr(),
+        kv_lens.data_ptr(), cu_q.data_ptr(), B, T, int(max_q_len), Hq, Hkv, D, k_pages.shape[0],
+        k_pages.shape[2], page_table.shape[1], strides, int(block_size),
+        D ** -0.5 if scale is None else float(scale), code, _code(out_dtype),
+        workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+        torch.cuda.current_stream(dev).cuda_stream))
+    return (o, lse) if return_lse else o
+
+
+def qkv_rope_paged_raw(qkv, n_heads: int, n_kv_heads: int, cos_table, sin_table, k_pages, v_pages,
+                       page_table, kv_lens, cu_q, q_out=None):
+    """Split a packed QKV projection, rotate q and k by their tokens' positions, write k and v
+    into the pages in place and q to q_out; returns q_out (tokens, n_heads, D).
+
+    qkv: (tokens, (n_heads + 2 * n_kv_heads) * D) with q, k, v heads in that order; cos_table,
+    sin_table: (max_pos, D / 2) fp32; the rest as paged_attn_raw (kv_lens counts the tokens
+    being written). The rotation is fp32, rounded once.
+    """
+    _check_cuda(qkv, cos_table, sin_table)
+    if qkv.dim() != 2 or qkv.shape[1] % (n_heads + 2 * n_kv_heads):
+        raise AssertionError("qkv must be (tokens, (n_heads + 2 * n_kv_heads) * head_dim)")
+    T = qkv.shape[0]
+    D = qkv.shape[1] // (n_heads + 2 * n_kv_heads)
+    B = _check_pages(k_pages, v_pages, page_table, kv_lens, cu_q, qkv.dtype, n_kv_heads, D)
+    if cos_table.dtype != torch.float32 or sin_table.dtype != torch.float32 \
+            or cos_table.shape != sin_table.shape or cos_table.shape[1:] != (D // 2,) \
+            or not cos_table.is_contiguous() or not sin_table.is_contiguous():
+        raise AssertionError("cos_table and sin_table must be contiguous (max_pos, head_dim / 2) fp32")
+    if qkv.stride(1) != 1 or qkv.stride(0) * qkv.element_size() % 16 or qkv.data_ptr() % 16:
+        qkv = qkv.clone(memory_format=torch.contiguous_format)
+    dev = qkv.device
+    if q_out is None:
+        q_out = torch.empty((T, n_heads, D), dtype=qkv.dtype, device=dev)
+    elif q_out.shape != (T, n_heads, D) or q_out.dtype != qkv.dtype or q_out.stride(2) != 1 \
+            or q_out.device != dev:
+        raise AssertionError("q_out must be (tokens, n_heads, head_dim) in qkv's dtype")
+    ks, vs = k_pages.stride(), v_pages.stride()
+    strides = i64_array((q_out.stride(0), q_out.stride(1), ks[0], ks[1], ks[2], vs[0], vs[1],
+                         vs[2], page_table.stride(0)))
+    check("bd3_qkv_rope_paged", _on_device(
+        dev, LIB.bd3_qkv_rope_paged, qkv.data_ptr(), qkv.stride(0), T, B, n_heads, n_kv_heads, D,
+        cos_table.data_ptr(), sin_table.data_ptr(), cos_table.shape[0], q_out.data_ptr(),
+        k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), kv_lens.data_ptr(),
+        cu_q.data_ptr(), k_pages.shape[0], k_pages.shape[2], page_table.shape[1], strides,
+        _code(qkv.dtype), torch.cuda.current_stream(dev).cuda_stream))
+    return q_out
+
+
+@torch.library.custom_op("bd3::paged_attn", mutates_args=("workspace",))
+def paged_attn_op(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                  page_table: torch.Tensor, kv_lens: torch.Tensor, cu_q: torch.Tensor,
+                  max_q_len: int, block_size: int, workspace: torch.Tensor) -> torch.Tensor:
+    return paged_attn_raw(q, k_pages, v_pages, page_table, kv_lens, cu_q, max_q_len, block_size,
+                          workspace=workspace)
+
+
+@paged_attn_op.register_fake
+def _(q, k_pages, v_pages, page_table, kv_lens, cu_q, max_q_len, block_size, workspace):
+    return q.new_empty(tuple(q.shape))
+
+
+@torch.library.custom_op("bd3::qkv_rope_paged", mutates_args=("k_pages", "v_pages"))
+def qkv_rope_paged_op(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, cos_table: torch.Tensor,
+                      sin_table: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                      page_table: torch.Tensor, kv_lens: torch.Tensor,
+                      cu_q: torch.Tensor) -> torch.Tensor:
+    """qkv_rope_paged_raw as a custom op: writes the pages in place, returns q."""
+    return qkv_rope_paged_raw(qkv, n_heads, n_kv_heads, cos_table, sin_table, k_pages, v_pages,
+                              page_table, kv_lens, cu_q)
+
+
+@qkv_rope_paged_op.register_fake
+def _(qkv, n_heads, n_kv_heads, cos_table, sin_table, k_pages, v_pages, page_table, kv_lens,
+      cu_q):
+    return qkv.new_empty((qkv.shape[0], n_heads, qkv.shape[1] // (n_heads + 2 * n_kv_heads)))
+
+
+# ---------------------------------------------------------------------------------------
 PROFILE_KERNELS = ("attn_fwd", "attn_prefill", "bwd_prep", "bwd_dq_convert", "bwd_fused",
                    "decode", "decode_combine", "qkv_rope_cache", "subs_sample")
 

@@ -17,6 +17,9 @@
 #include "decode.cuh"
 #include "f32_scale.cuh"
 #include "kv_rope.cuh"
+#include "logits.cuh"
+#include "paged_attn.cuh"
+#include "paged_rope.cuh"
 #include "peer_merge.cuh"
 #include "sampler.cuh"
 
@@ -1171,6 +1174,261 @@ int bd3_subs_sample_dev(const void* logits, const int64_t* logit_strides, int64_
   p.S = static_cast<int>(S);
   p.V = static_cast<int>(V);
   return launch_sample<true>(p, dtype, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"
+
+namespace {
+// What the paged entry points share: sizes of the page table and the pages.
+int check_pages(int64_t B, int64_t Hkv, int64_t num_pages, int64_t page_size, int64_t max_pages,
+                const void* page_table, const void* kv_lens, const void* cu_q) {
+  if (B < 1 || Hkv < 1) return fail(BD3_ERR_INVALID, "batch and heads must be >= 1");
+  if (num_pages < 1 || page_size < 1 || max_pages < 1)
+    return fail(BD3_ERR_INVALID, "pages, page size and pages per sequence must be >= 1");
+  if (num_pages > (1LL << 31) - 2 || max_pages > (1LL << 31) / page_size - 1 || B > (1LL << 30))
+    return fail(BD3_ERR_UNSUPPORTED, "more than 2^31 pages, or positions in a sequence");
+  if (page_table == nullptr || kv_lens == nullptr || cu_q == nullptr ||
+      reinterpret_cast<uintptr_t>(page_table) % 4 || reinterpret_cast<uintptr_t>(kv_lens) % 4 ||
+      reinterpret_cast<uintptr_t>(cu_q) % 4)
+    return fail(BD3_ERR_INVALID, "page_table, kv_lens and cu_q must be int32 device buffers");
+  return BD3_OK;
+}
+
+int64_t gcd64(int64_t a, int64_t b) { return b == 0 ? a : gcd64(b, a % b); }
+
+constexpr int kPagedCtas = 2;  // CTAs an SM of paged_attn_kernel
+
+// Counts (zero between calls), then the partials of the widest kernel's row tile.
+size_t paged_counter_bytes(int sms) { return static_cast<size_t>(2 * kPagedCtas * sms) * 4 + 256; }
+size_t paged_workspace_bytes(int sms) {
+  return paged_counter_bytes(sms) + static_cast<size_t>(2 * kPagedCtas * sms) * 32 * 66 * 4;
+}
+}  // namespace
+
+extern "C" {
+
+size_t bd3_paged_workspace_size(void) {
+  int sms = 0;
+  if (current_device_sms(&sms) != BD3_OK) return 0;
+  return paged_workspace_bytes(sms);
+}
+
+int bd3_paged_attn(const void* q, const void* k_pages, const void* v_pages, void* o, float* lse,
+                   const int32_t* page_table, const int32_t* kv_lens, const int32_t* cu_q,
+                   int64_t B, int64_t total_q, int64_t max_q, int64_t Hq, int64_t Hkv, int64_t D,
+                   int64_t num_pages, int64_t page_size, int64_t max_pages,
+                   const int64_t* strides, int64_t block_size, double scale, int dtype,
+                   int out_dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_pages(B, Hkv, num_pages, page_size, max_pages, page_table, kv_lens, cu_q);
+  if (rc != BD3_OK) return rc;
+  if (D != 64) return fail(BD3_ERR_UNSUPPORTED, "head_dim must be 64 (got %lld)", (long long)D);
+  if (dtype != BD3_BF16 && dtype != BD3_F16)
+    return fail(BD3_ERR_UNSUPPORTED, "inputs must be bf16 or f16 (dtype code %d)", dtype);
+  if (Hq < 1 || Hq % Hkv != 0 || Hkv > 65535)
+    return fail(BD3_ERR_INVALID, "query heads must be a multiple of the KV heads (%lld, %lld)",
+                (long long)Hq, (long long)Hkv);
+  if (page_size % 8 != 0)
+    return fail(BD3_ERR_UNSUPPORTED, "page_size must be a multiple of 8 (got %lld)",
+                (long long)page_size);
+  if (total_q < 0 || max_q < 0) return fail(BD3_ERR_INVALID, "total_q and max_q must be >= 0");
+  if (block_size < 1) return fail(BD3_ERR_INVALID, "block_size must be >= 1");
+  if (!(scale > 0.0) || scale > 1e30) return fail(BD3_ERR_INVALID, "scale must be positive and finite");
+  if (out_dtype != dtype && out_dtype != BD3_F32)
+    return fail(BD3_ERR_INVALID, "out_dtype must be the inputs' dtype or fp32");
+  if (total_q == 0 || max_q == 0) return BD3_OK;  // no new token
+  const int64_t G = Hq / Hkv;
+  if (max_q > total_q) max_q = total_q;
+  if (total_q > (1LL << 30) || max_q * G > (1LL << 30) || total_q * Hq > (1LL << 40))
+    return fail(BD3_ERR_UNSUPPORTED, "too many new tokens");
+  const int64_t oal = out_dtype == BD3_F32 ? 4 : 8;
+  if (q == nullptr || o == nullptr || reinterpret_cast<uintptr_t>(q) % 16 || strides[0] % 8 ||
+      strides[1] % 8 || reinterpret_cast<uintptr_t>(o) % 16 || strides[8] % oal ||
+      strides[9] % oal)
+    return fail(BD3_ERR_INVALID, "q and o: pointers and strides must be 16-byte aligned");
+  if (lse != nullptr && reinterpret_cast<uintptr_t>(lse) % 4)
+    return fail(BD3_ERR_INVALID, "lse must be a valid fp32 buffer");
+  if (workspace == nullptr) return fail(BD3_ERR_WORKSPACE, "paged attention needs its workspace");
+  int sms = 148;
+  if ((rc = ensure_context()) != BD3_OK || (rc = current_device_sms(&sms)) != BD3_OK) return rc;
+  if ( reinterpret_cast<uintptr_t>(workspace) % 16 ||
+      workspace_bytes < paged_workspace_bytes(sms))
+    return fail(BD3_ERR_WORKSPACE, "paged attention workspace: need %zu bytes, zeroed once",
+                paged_workspace_bytes(sms));
+  bd3::PagedParams p{};
+  p.q = q;
+  p.o = o;
+  p.lse = lse;
+  p.q_st = strides[0];
+  p.q_sh = strides[1];
+  p.o_st = strides[8];
+  p.o_sh = strides[9];
+  p.page_table = page_table;
+  p.pt_stride = strides[10];
+  p.kv_lens = kv_lens;
+  p.cu_q = cu_q;
+  p.counters = static_cast<int*>(workspace);
+  p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + paged_counter_bytes(sms));
+  p.B = static_cast<int>(B);
+  p.Hkv = static_cast<int>(Hkv);
+  p.G = static_cast<int>(G);
+  p.total_q = static_cast<int>(total_q);
+  p.max_q = static_cast<int>(max_q);
+  p.num_pages = static_cast<int>(num_pages);
+  p.page_size = static_cast<int>(page_size);
+  p.max_pages = static_cast<int>(max_pages);
+  p.bs = static_cast<int>(block_size < (1LL << 30) ? block_size : (1LL << 30));
+  p.out_f32 = out_dtype == BD3_F32;
+  p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
+  const int64_t rows = max_q * G;
+  const int64_t tile_rows = rows > 16 ? 32 : 16;
+  p.row_tiles = static_cast<int>((rows + tile_rows - 1) / tile_rows);
+  if (B * p.row_tiles > (1LL << 30)) return fail(BD3_ERR_UNSUPPORTED, "too many row tiles");
+  p.box = static_cast<int>(gcd64(page_size, bd3::kPgBN));
+  p.min_chunk = 1;
+  CUtensorMap tk, tv;
+  if ((rc = make_map(&tk, k_pages, dtype, page_size, Hkv, num_pages, strides + 2, p.box, "k_pages")) != BD3_OK) return rc;
+  if ((rc = make_map(&tv, v_pages, dtype, page_size, Hkv, num_pages, strides + 5, p.box, "v_pages")) != BD3_OK) return rc;
+  const int64_t tiles = (max_pages * page_size + bd3::kPgBN - 1) / bd3::kPgBN;
+  const int64_t most = B * p.row_tiles * Hkv;
+  int64_t grid = kPagedCtas * sms;
+  if (most < grid && most * tiles < grid) grid = most * tiles;
+  const bool bf = dtype == BD3_BF16;
+  auto kern = tile_rows == 16 ? (bf ? bd3::paged_attn_kernel<1, true> : bd3::paged_attn_kernel<1, false>)
+                              : (bf ? bd3::paged_attn_kernel<2, true> : bd3::paged_attn_kernel<2, false>);
+  const uint32_t smem = tile_rows == 16 ? bd3::PgSmem<1>::kAlloc : bd3::PgSmem<2>::kAlloc;
+  if ((rc = set_smem(kern, smem, 20 + (tile_rows == 16 ? 0 : 2) + (bf ? 0 : 1))) != BD3_OK) return rc;
+  return launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(bd3::kPgThreads), smem,
+                    static_cast<cudaStream_t>(stream), "paged_attn_kernel launch", tk, tv, p);
+}
+
+int bd3_qkv_rope_paged(const void* qkv, int64_t qkv_stride, int64_t T, int64_t B, int64_t Hq,
+                       int64_t Hkv, int64_t D, const float* cos_table, const float* sin_table,
+                       int64_t max_pos, void* q_out, void* k_pages, void* v_pages,
+                       const int32_t* page_table, const int32_t* kv_lens, const int32_t* cu_q,
+                       int64_t num_pages, int64_t page_size, int64_t max_pages,
+                       const int64_t* strides, int dtype, void* stream) {
+  int rc = check_pages(B, Hkv, num_pages, page_size, max_pages, page_table, kv_lens, cu_q);
+  if (rc != BD3_OK) return rc;
+  if (Hq < 1) return fail(BD3_ERR_INVALID, "query heads must be >= 1");
+  if (dtype != BD3_BF16 && dtype != BD3_F16 && dtype != BD3_F32)
+    return fail(BD3_ERR_UNSUPPORTED, "bad dtype code %d", dtype);
+  if (D < 16 || D % 16 != 0 || D > 1024)
+    return fail(BD3_ERR_UNSUPPORTED, "head_dim must be a multiple of 16 up to 1024 (got %lld)", (long long)D);
+  if (T < 0 || T > (1LL << 30) || Hq > 65536 || Hkv > 65536)
+    return fail(BD3_ERR_INVALID, "bad token or head count");
+  if (cos_table == nullptr || sin_table == nullptr || max_pos < 1 ||
+      reinterpret_cast<uintptr_t>(cos_table) % 16 || reinterpret_cast<uintptr_t>(sin_table) % 16)
+    return fail(BD3_ERR_INVALID, "RoPE tables must be 16-byte aligned fp32 buffers");
+  if (T == 0) return BD3_OK;
+  const int64_t al = 16 / static_cast<int64_t>(elem_bytes(dtype));
+  const void* ptr[4] = {qkv, q_out, k_pages, v_pages};
+  for (const void* x : ptr)
+    if (x == nullptr || reinterpret_cast<uintptr_t>(x) % 16)
+      return fail(BD3_ERR_INVALID, "qkv, q_out and the pages must be 16-byte aligned");
+  for (int i = 0; i < 8; ++i)
+    if (strides[i] % al) return fail(BD3_ERR_INVALID, "strides must be multiples of 16 bytes");
+  if (qkv_stride % al) return fail(BD3_ERR_INVALID, "strides must be multiples of 16 bytes");
+  int sms = 148;
+  if ((rc = ensure_context()) != BD3_OK || (rc = current_device_sms(&sms)) != BD3_OK) return rc;
+  bd3::PagedRopeParams p{};
+  p.qkv = qkv;
+  p.qkv_st = qkv_stride;
+  p.cos_table = cos_table;
+  p.sin_table = sin_table;
+  p.max_pos = max_pos;
+  p.q_out = q_out;
+  p.q_st = strides[0];
+  p.q_sh = strides[1];
+  p.k_pages = k_pages;
+  p.k_sp = strides[2];
+  p.k_sh = strides[3];
+  p.k_sr = strides[4];
+  p.v_pages = v_pages;
+  p.v_sp = strides[5];
+  p.v_sh = strides[6];
+  p.v_sr = strides[7];
+  p.page_table = page_table;
+  p.pt_stride = strides[8];
+  p.kv_lens = kv_lens;
+  p.cu_q = cu_q;
+  p.B = static_cast<int>(B);
+  p.T = static_cast<int>(T);
+  p.Hq = static_cast<int>(Hq);
+  p.Hkv = static_cast<int>(Hkv);
+  p.D = static_cast<int>(D);
+  p.num_pages = static_cast<int>(num_pages);
+  p.page_size = static_cast<int>(page_size);
+  p.max_pages = static_cast<int>(max_pages);
+  p.tpb = 4;
+  auto kern = dtype == BD3_BF16  ? bd3::qkv_rope_paged_kernel<0>
+              : dtype == BD3_F16 ? bd3::qkv_rope_paged_kernel<1>
+                                 : bd3::qkv_rope_paged_kernel<2>;
+  const int64_t grid = (T + p.tpb - 1) / p.tpb;
+  return launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(256), 0,
+                    static_cast<cudaStream_t>(stream), "qkv_rope_paged_kernel launch", p);
+}
+
+int bd3_process_logits(const void* logits, void* out, const int64_t* strides, int64_t B,
+                       int64_t S, int64_t V, const void* history, int history_is_i32,
+                       int64_t history_stride, int64_t history_cap, const int32_t* history_len,
+                       const float* repetition, const float* presence, const float* frequency,
+                       const float* bias, int64_t bias_stride, const uint32_t* allowed,
+                       const int64_t* allowed_strides, int dtype, void* stream) {
+  if (B < 1 || S < 1 || V < 1) return fail(BD3_ERR_INVALID, "batch, rows and vocabulary must be >= 1");
+  if (dtype != BD3_BF16 && dtype != BD3_F16 && dtype != BD3_F32)
+    return fail(BD3_ERR_UNSUPPORTED, "bad dtype code %d", dtype);
+  if (V > (1LL << 30) || S > (1LL << 30) || B > 65535)
+    return fail(BD3_ERR_UNSUPPORTED, "at most 65535 sequences and 2^30 rows or tokens");
+  const uintptr_t es = elem_bytes(dtype);
+  if (logits == nullptr || out == nullptr || reinterpret_cast<uintptr_t>(logits) % es ||
+      reinterpret_cast<uintptr_t>(out) % es)
+    return fail(BD3_ERR_INVALID, "logits and out must be device buffers of their dtype");
+  if (history != nullptr &&
+      (history_len == nullptr || history_cap < 0 || history_cap > (1LL << 30) ||
+       reinterpret_cast<uintptr_t>(history) % (history_is_i32 ? 4 : 8)))
+    return fail(BD3_ERR_INVALID, "history needs its lengths (int32) and at most 2^30 entries");
+  if (allowed != nullptr && allowed_strides == nullptr)
+    return fail(BD3_ERR_INVALID, "allowed needs its strides");
+  int rc, sms = 148;
+  if ((rc = ensure_context()) != BD3_OK || (rc = current_device_sms(&sms)) != BD3_OK) return rc;
+  bd3::LogitParams p{};
+  p.logits = logits;
+  p.out = out;
+  p.l_sb = strides[0];
+  p.l_ss = strides[1];
+  p.o_sb = strides[2];
+  p.o_ss = strides[3];
+  p.history = history_cap > 0 ? history : nullptr;
+  p.h_sb = history_stride;
+  p.hist_len = history_len;
+  p.hist32 = history_is_i32;
+  p.hist_cap = static_cast<int>(history_cap);
+  p.repetition = repetition;
+  p.presence = presence;
+  p.frequency = frequency;
+  p.bias = bias;
+  p.bias_sb = bias_stride;
+  p.allowed = allowed;
+  p.a_sb = allowed != nullptr ? allowed_strides[0] : 0;
+  p.a_ss = allowed != nullptr ? allowed_strides[1] : 0;
+  p.B = static_cast<int>(B);
+  p.S = static_cast<int>(S);
+  p.V = static_cast<int>(V);
+  const int64_t span = (V + 14) / 8 * 8;  // chunks of 8 that start up to 7 logits early
+  p.slice = 4096;
+  while (p.slice > 1024 && (span + p.slice - 1) / p.slice * B < 2 * sms) p.slice /= 2;
+  p.n_slices = static_cast<int>((span + p.slice - 1) / p.slice);
+  p.rows = static_cast<int>(S);
+  while (p.rows > 1 && p.n_slices * B * ((S + p.rows - 1) / p.rows) < 2 * sms) p.rows = (p.rows + 1) / 2;
+  auto kern = dtype == BD3_BF16  ? bd3::logits_kernel<0>
+              : dtype == BD3_F16 ? bd3::logits_kernel<1>
+                                 : bd3::logits_kernel<2>;
+  const int64_t z = (S + p.rows - 1) / p.rows;
+  if (z > 65535) return fail(BD3_ERR_UNSUPPORTED, "too many rows");
+  const uint32_t smem = static_cast<uint32_t>(bd3::logit_smem_words(p.slice)) * 4;
+  return launch_pdl(kern, dim3(static_cast<unsigned>(p.n_slices), static_cast<unsigned>(B), static_cast<unsigned>(z)),
+                    dim3(bd3::kLogitThreads), smem, static_cast<cudaStream_t>(stream),
+                    "logits_kernel launch", p);
 }
 
 int bd3_profile_enable(int on) {

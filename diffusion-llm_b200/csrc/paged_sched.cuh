@@ -1,0 +1,255 @@
+// Work distribution of attention over a paged KV cache (sm_100a), shared by its two kernels.
+//
+// The new tokens of all sequences are packed; sequence b has the rows [cu_q[b], cu_q[b+1]) and
+// they are the last of its kv_lens[b] positions. A token at position p sees the keys
+// [0, min((p / bs + 1) * bs, kv_len)): block-causal attention, causal for bs = 1. The G = Hq/Hkv
+// query heads that share a KV head are folded into the row index, r = token * G + g, so a
+// KV head's keys are read once for all of them.
+//
+// Work is a list of items (sequence b, row tile i, KV head h), each with n(b, i) key tiles, laid
+// end to end in that order; W is its length in key tiles. The lengths live on the device (a
+// captured launch serves every step of a growing batch), so each CTA computes the prefix sums
+// of n itself: the threads sum n * Hkv over their share of the (b, i) pairs, a block scan gives
+// every share's start. CTA c then takes tiles [c * chunk, (c + 1) * chunk) of the list,
+// chunk = max(ceil(W / CTAs), a minimum): the same number of tiles for every CTA whatever
+// the mix of lengths, so one 64K-token sequence among short ones does not set the time.
+// An item cut by chunk borders leaves one partial (m, l, unnormalised O) per CTA in the
+// workspace; the CTA that finishes last (an atomic count per cut item) merges the partials in
+// CTA order, so the sum's order does not depend on timing. Nothing waits for another CTA. The
+// counts are zero before the first call (the caller's zeroed workspace) and the merging CTA
+// sets its count back to zero, so calls in stream order share one workspace.
+#pragma once
+
+#include "common.cuh"
+#include "tile_ranges.h"
+
+namespace bd3 {
+
+struct PagedParams {
+  const void* q;              // (total_q, Hq, 64); token and head strides in elements
+  void* o;                    // (total_q, Hq, 64) in the output dtype
+  float* lse;                 // optional (total_q, Hq) contiguous natural-log LSE
+  long long q_st, q_sh, o_st, o_sh;
+  const int* page_table;      // (B, max_pages): page of positions [j * page_size, ...)
+  long long pt_stride;
+  const int* kv_lens;         // (B)
+  const int* cu_q;            // (B + 1)
+  int* counters;              // 2 per CTA, zero between calls
+  float* partials;            // 2 slots per CTA of (m, l, O) of a row tile
+  int B, Hkv, G, total_q, max_q;
+  int num_pages, page_size, max_pages;
+  int box;                    // rows of one TMA piece: divides the page size and the key tile
+  int bs;
+  int row_tiles;              // row tiles of max_q tokens
+  int min_chunk;              // key tiles that a CTA takes at least
+  int out_f32;
+  float scale_log2;           // softmax scale * log2(e)
+};
+
+// Sequence b as the kernels use it: its first packed row, its new tokens and its keys. Values
+// outside the call's own bounds are cut to them (no address depends on the uncut ones).
+struct PagedSeq {
+  int q0, qn, kv;
+  bool bad;
+};
+__device__ __forceinline__ PagedSeq paged_seq(const PagedParams& p, int b) {
+  const int a = p.cu_q[b], e = p.cu_q[b + 1], kv = p.kv_lens[b];
+  const long long cap = static_cast<long long>(p.max_pages) * p.page_size;
+  PagedSeq s;
+  s.q0 = imin(a < 0 ? 0 : a, p.total_q);
+  s.qn = e > s.q0 ? imin(e, p.total_q) - s.q0 : 0;
+  s.qn = s.qn < 0 ? 0 : imin(s.qn, p.max_q);
+  s.kv = kv < 0 ? 0 : (kv > cap ? static_cast<int>(cap) : kv);
+  s.bad = s.q0 != a || s.qn != e - a || s.kv != kv;
+  return s;
+}
+
+// Exclusive end of the keys that new token t of the sequence sees (0: none).
+__device__ __forceinline__ int paged_hi(const PagedParams& p, const PagedSeq& s, int t) {
+  const int pos = s.kv - s.qn + t;
+  if (pos < 0) return 0;
+  const long long hi = (static_cast<long long>(pos / p.bs) + 1) * p.bs;
+  return hi < s.kv ? static_cast<int>(hi) : s.kv;
+}
+
+// Key tiles of row tile i: up to the last key that its last row sees; 0 past the sequence's rows
+// and 1 for rows that see no key (their output is written too).
+template <int kBM, int kBN>
+__device__ __forceinline__ int paged_tiles(const PagedParams& p, const PagedSeq& s, int i,
+                                           int* hi_out) {
+  const int rows = s.qn * p.G, r0 = i * kBM;
+  if (r0 >= rows) return 0;
+  const int hi = paged_hi(p, s, (imin(r0 + kBM, rows) - 1) / p.G);
+  *hi_out = hi;
+  return hi > kBN ? (hi - 1) / kBN + 1 : 1;
+}
+
+// One CTA's share of an item.
+struct PagedItem {
+  PagedSeq s;
+  int b, i, h;
+  int hi;         // exclusive end of the keys that any row of the item sees
+  int t0, t1;     // key tiles of this share
+  int parts;      // CTAs that share the item; 1: this one alone
+  int slot;       // this share's partial
+  int slot0;      // the first share's partial, and the item's count
+  int cta0;       // the first share's CTA
+};
+
+struct PagedCursor {
+  int b, i;
+  long long base;             // list position of the pair (b, i)'s first tile
+  long long pos, lo, end, chunk;
+};
+
+// The next share of this CTA's chunk; false at its end.
+template <int kBM, int kBN>
+__device__ __forceinline__ bool paged_next(const PagedParams& p, PagedCursor& c, PagedItem& it) {
+  while (c.pos < c.end && c.b < p.B) {
+    it.s = paged_seq(p, c.b);
+    const int n = paged_tiles<kBM, kBN>(p, it.s, c.i, &it.hi);
+    if (n == 0) {  // past the sequence's rows
+      ++c.b;
+      c.i = 0;
+      continue;
+    }
+    const long long w = static_cast<long long>(n) * p.Hkv;
+    if (c.pos >= c.base + w) {
+      c.base += w;
+      if (++c.i == p.row_tiles) {
+        ++c.b;
+        c.i = 0;
+      }
+      continue;
+    }
+    it.b = c.b;
+    it.i = c.i;
+    it.h = static_cast<int>((c.pos - c.base) / n);
+    const long long start = c.base + static_cast<long long>(it.h) * n;  // the item's first tile
+    it.t0 = static_cast<int>(c.pos - start);
+    const long long left = c.end - c.pos;
+    it.t1 = left < n - it.t0 ? it.t0 + static_cast<int>(left) : n;
+    const long long c0 = start / c.chunk, c1 = (start + n - 1) / c.chunk;
+    it.cta0 = static_cast<int>(c0);
+    it.parts = static_cast<int>(c1 - c0) + 1;
+    it.slot0 = 2 * it.cta0 + (start == c0 * c.chunk ? 0 : 1);
+    it.slot = 2 * static_cast<int>(blockIdx.x) + (c.pos == c.lo ? 0 : 1);
+    c.pos += it.t1 - it.t0;
+    return true;
+  }
+  return false;
+}
+// Partial slot of share j of an item.
+__device__ __forceinline__ int paged_part_slot(const PagedItem& it, int j) {
+  return j == 0 ? it.slot0 : 2 * (it.cta0 + j);
+}
+
+struct PagedScan {
+  long long warp_sum[32];
+  long long base;
+  int b, i;
+};
+
+// This CTA's chunk of the list, found by all kThreads threads; ends with a barrier. The chunk
+// is empty (pos == end) for a CTA past the list.
+template <int kThreads, int kBM, int kBN>
+__device__ __forceinline__ PagedCursor paged_chunk(const PagedParams& p, PagedScan* sc) {
+  const int pairs = p.B * p.row_tiles;
+  const int per = cdiv(pairs, kThreads);
+  const int e0 = imin(static_cast<int>(threadIdx.x) * per, pairs), e1 = imin(e0 + per, pairs);
+  auto tiles = [&](int e) -> long long {
+    const PagedSeq s = paged_seq(p, e / p.row_tiles);
+    if (s.bad && blockIdx.x == 0) atomicOr(&g_bd3_status, kStatusBadLaunch);
+    int hi;
+    return static_cast<long long>(paged_tiles<kBM, kBN>(p, s, e % p.row_tiles, &hi)) * p.Hkv;
+  };
+  long long mine = 0;
+  for (int e = e0; e < e1; ++e) mine += tiles(e);
+  const int lane = static_cast<int>(lane_id()), w = static_cast<int>(threadIdx.x) >> 5;
+  long long incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += y;
+  }
+  if (lane == 31) sc->warp_sum[w] = incl;
+  __syncthreads();
+  long long before = 0, total = 0;
+#pragma unroll
+  for (int k = 0; k < kThreads / 32; ++k) {
+    if (k == w) before = total;
+    total += sc->warp_sum[k];
+  }
+  PagedCursor c;
+  c.chunk = (total + gridDim.x - 1) / gridDim.x;
+  if (c.chunk < p.min_chunk) c.chunk = p.min_chunk;
+  c.lo = c.chunk * blockIdx.x;
+  c.end = c.lo + c.chunk < total ? c.lo + c.chunk : total;
+  c.pos = c.lo < c.end ? c.lo : c.end;
+  long long at = before + incl - mine;
+  if (c.lo >= at && c.lo < at + mine) {  // this thread's share holds the chunk's start
+    for (int e = e0; e < e1; ++e) {
+      const long long n = tiles(e);
+      if (c.lo < at + n) {
+        sc->base = at;
+        sc->b = e / p.row_tiles;
+        sc->i = e % p.row_tiles;
+        break;
+      }
+      at += n;
+    }
+  }
+  __syncthreads();
+  c.base = sc->base;
+  c.b = sc->b;
+  c.i = sc->i;
+  if (c.pos >= c.end) c.b = p.B;
+  return c;
+}
+
+// Pages of the kBN / box pieces of key tiles, looked up by a whole warp ahead of their use: lane
+// l holds piece l % pieces of tile l / pieces of a batch of 32 / pieces tiles. Pieces past the
+// visible keys get page num_pages, which is outside the tensor map: the TMA fills their rows
+// with zeros and reads nothing. A page id outside [0, num_pages) is treated the same way and
+// sets status bit 2.
+template <int kBN>
+__device__ __forceinline__ int paged_lookup(const PagedParams& p, const PagedItem& it, int tile,
+                                            int* row) {
+  const int pieces = kBN / p.box, lane = static_cast<int>(lane_id());
+  const long long key = static_cast<long long>(tile + lane / pieces) * kBN + (lane % pieces) * p.box;
+  *row = 0;
+  if (key >= it.hi) return p.num_pages;
+  const int pg = static_cast<int>(key) / p.page_size;
+  *row = static_cast<int>(key) - pg * p.page_size;
+  const int id = p.page_table[it.b * p.pt_stride + pg];
+  if (id < 0 || id >= p.num_pages) {
+    atomicOr(&g_bd3_status, kStatusBadLaunch);
+    return p.num_pages;
+  }
+  return id;
+}
+
+// Stream K and V pieces of the item's key tiles [t0, t1) into a ring, whole warp: stage(J) waits
+// for ring slot J and returns the K destination (0: gave up), V follows at `v_off`.
+// (The two kernels differ in their rings, so they pass the waits and barriers in.)
+template <int kBN, typename Wait, typename Issue>
+__device__ __forceinline__ bool paged_stream(const PagedParams& p, const PagedItem& it, int& J,
+                                             Wait&& wait, Issue&& issue) {
+  const int pieces = kBN / p.box, per = 32 / pieces, lane = static_cast<int>(lane_id());
+  int row, row_next = 0, id_next = 0;
+  int id = paged_lookup<kBN>(p, it, it.t0, &row);
+  for (int t = it.t0; t < it.t1; t += per) {
+    if (t + per < it.t1) id_next = paged_lookup<kBN>(p, it, t + per, &row_next);
+    const int m = imin(per, it.t1 - t);
+    for (int k = 0; k < m; ++k, ++J) {
+      if (!wait(J)) return false;
+      __syncwarp();
+      if (lane / pieces == k) issue(J, lane % pieces, id, row);
+    }
+    id = id_next;
+    row = row_next;
+  }
+  return true;
+}
+
+}  // namespace bd3

@@ -276,6 +276,88 @@ BD3_API int bd3_subs_sample_dev(const void* logits, const int64_t* logit_strides
                                 int dtype, void* stream);
 
 /* ---------------------------------------------------------------------------------------
+ * Paged KV cache: attention of packed new tokens over it, and the fused write into it (no
+ * counterpart in the reference, whose cache is one contiguous tensor per layer,
+ * model/kv_cache.py:9-55).
+ *   k_pages, v_pages: (num_pages, Hkv, page_size, D), any 16-byte-multiple strides (the
+ *     page-row-head order included), D contiguous. Position p of sequence b sits at row
+ *     p % page_size of page page_table[b][p / page_size].
+ *   page_table: device int32 (B, max_pages), rows contiguous; entries past a sequence's pages
+ *     are not read.
+ *   cu_q: device int32 (B + 1), kv_lens: device int32 (B). The new tokens of all sequences are
+ *     packed: sequence b has rows [cu_q[b], cu_q[b+1]) and they are the last of its kv_lens[b]
+ *     positions (the new tokens counted). A sequence may have no new tokens. Rows at or past
+ *     cu_q[B] belong to no sequence and are left alone.
+ *
+ * bd3_paged_attn: block-causal attention of the new tokens: a token at position p sees the
+ * positions [0, min((p / block_size + 1) * block_size, kv_len)) of its sequence (the rule of
+ * bd3_decode_attn; block_size 1 is causal, block_size >= kv_len bidirectional). A token that
+ * sees none (kv_len below the new tokens' count) gets O = 0 and LSE = -inf. Query heads h share
+ * KV head h / (Hq / Hkv). What lies in a page past kv_len is never used (NaN included).
+ *   q, o: (total_q, Hq, 64), o in dtype or fp32; lse: optional (total_q, Hq) fp32 contiguous.
+ *   max_q: the most new tokens of a sequence (host). page_size % 8 == 0.
+ *   strides[11] = q (token, head), k_pages, v_pages (page, head, row), o (token, head),
+ *     page_table (sequence), in elements. scale: of the scores, usually 1 / sqrt(D).
+ *   workspace: bd3_paged_workspace_size() bytes on the current device, zeroed once by the
+ *     caller before its first use; every call leaves it ready for the next. Calls that share
+ *     one must be ordered (the same stream, or events); after device status bit 1 zero it
+ *     again.
+ * Lengths, offsets or page ids outside the call's bounds are cut to them (nothing out of
+ * bounds is read or written) and set device status bit 2. The launch depends on the sizes
+ * only, so a captured CUDA graph serves changing lengths and tables.
+ *
+ * bd3_qkv_rope_paged: splits the projection's rows (T, (Hq + 2 Hkv) * D; q, k, v heads in that
+ * order, row stride qkv_stride), rotates q and k by their token's position (rotate-half RoPE,
+ * tables (max_pos, D/2) fp32; fp32 arithmetic, rounded once) and writes q to q_out and k, v
+ * into the pages. dtype: BD3_BF16, BD3_F16 or BD3_F32, the pages' included. D % 16 == 0.
+ *   strides[9] = q_out (token, head), k_pages, v_pages (page, head, row), page_table
+ *     (sequence), in elements.
+ * A token whose position lies outside [0, max_pos) or the page table, or whose page id is
+ * outside [0, num_pages), is left unwritten and sets device status bit 4. Two sequences must
+ * not write the same row. */
+BD3_API size_t bd3_paged_workspace_size(void);
+BD3_API int bd3_paged_attn(const void* q, const void* k_pages, const void* v_pages, void* o,
+                           float* lse, const int32_t* page_table, const int32_t* kv_lens,
+                           const int32_t* cu_q, int64_t B, int64_t total_q, int64_t max_q,
+                           int64_t Hq, int64_t Hkv, int64_t D, int64_t num_pages,
+                           int64_t page_size, int64_t max_pages, const int64_t* strides,
+                           int64_t block_size, double scale, int dtype, int out_dtype,
+                           void* workspace, size_t workspace_bytes, void* stream);
+BD3_API int bd3_qkv_rope_paged(const void* qkv, int64_t qkv_stride, int64_t T, int64_t B,
+                               int64_t Hq, int64_t Hkv, int64_t D, const float* cos_table,
+                               const float* sin_table, int64_t max_pos, void* q_out,
+                               void* k_pages, void* v_pages, const int32_t* page_table,
+                               const int32_t* kv_lens, const int32_t* cu_q, int64_t num_pages,
+                               int64_t page_size, int64_t max_pages, const int64_t* strides,
+                               int dtype, void* stream);
+
+/* Penalties for repeated tokens, a bias and a grammar mask on a step's logits, in one pass (no
+ * counterpart in the reference, whose sampler takes the backbone's logits as they are,
+ * sample/sampler.py:100-122). With n the occurrences of token v in the first history_len[b]
+ * entries of history[b]:
+ *   x = logits[b, s, v];  if n > 0: x = (x > 0 ? x / repetition[b] : x * repetition[b])
+ *                                       - (frequency[b] * n + presence[b])
+ *   x += bias[v];  x = -inf if bit v % 32 of allowed word v / 32 is 0
+ * in fp32, rounded once to dtype.
+ *   logits, out: (B, S, V) in dtype (BD3_BF16, BD3_F16, BD3_F32), vocabulary contiguous; out may
+ *     be logits; strides[4] = logits, out (batch, row) in elements.
+ *   history: device int64 (int32 with history_is_i32) (B, history_cap), row stride
+ *     history_stride, or NULL; tokens outside [0, V) are ignored; history_len: int32 (B), cut
+ *     to [0, history_cap].
+ *   repetition (> 0), presence, frequency: device fp32 (B), or NULL for 1, 0, 0.
+ *   bias: device fp32 (V), bias_stride 0, or (B, V); or NULL.
+ *   allowed: device uint32 words, ceil(V / 32) per row, strides (batch, row) with 0 where rows
+ *     share them; or NULL. Logits of eight forbidden tokens in a row may not be read.
+ * A row whose tokens are all forbidden becomes -inf throughout: a sampler has nothing to draw. */
+BD3_API int bd3_process_logits(const void* logits, void* out, const int64_t* strides, int64_t B,
+                               int64_t S, int64_t V, const void* history, int history_is_i32,
+                               int64_t history_stride, int64_t history_cap,
+                               const int32_t* history_len, const float* repetition,
+                               const float* presence, const float* frequency, const float* bias,
+                               int64_t bias_stride, const uint32_t* allowed,
+                               const int64_t* allowed_strides, int dtype, void* stream);
+
+/* ---------------------------------------------------------------------------------------
  * Per-kernel timing for benchmarks. While enabled, every launch is bracketed by a pair of
  * CUDA events on its own stream (at most 8192 launches are kept). bd3_profile_collect()
  * waits for them and writes, per kernel id (0 training forward, 1 prefill forward, 2 backward
