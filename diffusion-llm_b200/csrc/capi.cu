@@ -19,6 +19,7 @@
 #include "kv_rope.cuh"
 #include "logits.cuh"
 #include "paged_attn.cuh"
+#include "paged_attn_tc.cuh"
 #include "paged_rope.cuh"
 #include "peer_merge.cuh"
 #include "sampler.cuh"
@@ -1196,12 +1197,17 @@ int check_pages(int64_t B, int64_t Hkv, int64_t num_pages, int64_t page_size, in
 
 int64_t gcd64(int64_t a, int64_t b) { return b == 0 ? a : gcd64(b, a % b); }
 
-constexpr int kPagedCtas = 2;  // CTAs an SM of paged_attn_kernel
+constexpr int kPagedCtas = 2;  // CTAs an SM of paged_attn_kernel (paged_attn_tc_kernel: 1)
+
+// Rows per sequence and KV head up to which paged_attn_kernel takes a call.
+constexpr int64_t kPagedMaxRows = 32;
 
 // Counts (zero between calls), then the partials of the widest kernel's row tile.
 size_t paged_counter_bytes(int sms) { return static_cast<size_t>(2 * kPagedCtas * sms) * 4 + 256; }
 size_t paged_workspace_bytes(int sms) {
-  return paged_counter_bytes(sms) + static_cast<size_t>(2 * kPagedCtas * sms) * 32 * 66 * 4;
+  const size_t rows = static_cast<size_t>(2 * kPagedCtas * sms) * 32 * 66 * 4;
+  const size_t tc = static_cast<size_t>(2 * sms) * bd3::kPtSlot * 4;
+  return paged_counter_bytes(sms) + (rows > tc ? rows : tc);
 }
 }  // namespace
 
@@ -1280,25 +1286,31 @@ int bd3_paged_attn(const void* q, const void* k_pages, const void* v_pages, void
   p.out_f32 = out_dtype == BD3_F32;
   p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
   const int64_t rows = max_q * G;
-  const int64_t tile_rows = rows > 16 ? 32 : 16;
-  p.row_tiles = static_cast<int>((rows + tile_rows - 1) / tile_rows);
+  const int64_t bm = rows > kPagedMaxRows ? bd3::kPtBM : rows > 16 ? 32 : 16;
+  const int bn = bm == bd3::kPtBM ? bd3::kPtBN : bd3::kPgBN;
+  p.row_tiles = static_cast<int>((rows + bm - 1) / bm);
   if (B * p.row_tiles > (1LL << 30)) return fail(BD3_ERR_UNSUPPORTED, "too many row tiles");
-  p.box = static_cast<int>(gcd64(page_size, bd3::kPgBN));
+  p.box = static_cast<int>(gcd64(page_size, bn));
   p.min_chunk = 1;
   CUtensorMap tk, tv;
   if ((rc = make_map(&tk, k_pages, dtype, page_size, Hkv, num_pages, strides + 2, p.box, "k_pages")) != BD3_OK) return rc;
   if ((rc = make_map(&tv, v_pages, dtype, page_size, Hkv, num_pages, strides + 5, p.box, "v_pages")) != BD3_OK) return rc;
-  const int64_t tiles = (max_pages * page_size + bd3::kPgBN - 1) / bd3::kPgBN;
-  const int64_t most = B * p.row_tiles * Hkv;
-  int64_t grid = kPagedCtas * sms;
+  // one CTA per resident slot, fewer when there cannot be as many key tiles
+  const int64_t most = B * p.row_tiles * Hkv, tiles = (max_pages * page_size + bn - 1) / bn;
+  int64_t grid = bm == bd3::kPtBM ? sms : kPagedCtas * sms;
   if (most < grid && most * tiles < grid) grid = most * tiles;
   const bool bf = dtype == BD3_BF16;
-  auto kern = tile_rows == 16 ? (bf ? bd3::paged_attn_kernel<1, true> : bd3::paged_attn_kernel<1, false>)
-                              : (bf ? bd3::paged_attn_kernel<2, true> : bd3::paged_attn_kernel<2, false>);
-  const uint32_t smem = tile_rows == 16 ? bd3::PgSmem<1>::kAlloc : bd3::PgSmem<2>::kAlloc;
-  if ((rc = set_smem(kern, smem, 20 + (tile_rows == 16 ? 0 : 2) + (bf ? 0 : 1))) != BD3_OK) return rc;
-  return launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(bd3::kPgThreads), smem,
-                    static_cast<cudaStream_t>(stream), "paged_attn_kernel launch", tk, tv, p);
+  void (*kern)(const CUtensorMap, const CUtensorMap, const bd3::PagedParams) =
+      bm == 16   ? (bf ? bd3::paged_attn_kernel<1, true> : bd3::paged_attn_kernel<1, false>)
+      : bm == 32 ? (bf ? bd3::paged_attn_kernel<2, true> : bd3::paged_attn_kernel<2, false>)
+                 : (bf ? bd3::paged_attn_tc_kernel<true> : bd3::paged_attn_tc_kernel<false>);
+  const uint32_t smem = bm == 16   ? bd3::PgSmem<1>::kAlloc
+                        : bm == 32 ? bd3::PgSmem<2>::kAlloc
+                                   : bd3::PtSmem::kAlloc;
+  const unsigned threads = bm == bd3::kPtBM ? bd3::kPtThreads : bd3::kPgThreads;
+  if ((rc = set_smem(kern, smem, (bm == 16 ? 0 : bm == 32 ? 2 : 4) + (bf ? 0 : 1))) != BD3_OK) return rc;
+  return launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(threads), smem,
+                    static_cast<cudaStream_t>(stream), "paged attention launch", tk, tv, p);
 }
 
 int bd3_qkv_rope_paged(const void* qkv, int64_t qkv_stride, int64_t T, int64_t B, int64_t Hq,

@@ -316,16 +316,16 @@ __global__ void __launch_bounds__(kPgThreads, 2)
     }
     if (it.parts > 1) {
       // the share that finishes last merges the item's partials, in CTA order
-      __threadfence();
       asm volatile("bar.sync 1, 128;" ::: "memory");
       if (threadIdx.x == 0) {
+        __threadfence();
         const int before = atomicAdd(&p.counters[it.slot0], 1);
         *last_flag = before == it.parts - 1;
         if (before == it.parts - 1) p.counters[it.slot0] = 0;
+        __threadfence();
       }
       asm volatile("bar.sync 1, 128;" ::: "memory");
       if (*last_flag) {
-        __threadfence();
         for (int idx = threadIdx.x; idx < kRows * 8; idx += 128) {
           const int rl = idx >> 3, c8 = (idx & 7) * 8;
           const int r = r0 + rl;
