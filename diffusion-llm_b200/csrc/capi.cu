@@ -1206,7 +1206,7 @@ constexpr int64_t kPagedMaxRows = 32;
 size_t paged_counter_bytes(int sms) { return static_cast<size_t>(2 * kPagedCtas * sms) * 4 + 256; }
 size_t paged_workspace_bytes(int sms) {
   const size_t rows = static_cast<size_t>(2 * kPagedCtas * sms) * 32 * 66 * 4;
-  const size_t tc = static_cast<size_t>(2 * sms) * bd3::kPtSlot * 4;
+  const size_t tc = static_cast<size_t>(2 * 2 * sms) * bd3::kPtSlot * 4;
   return paged_counter_bytes(sms) + (rows > tc ? rows : tc);
 }
 }  // namespace
@@ -1289,7 +1289,8 @@ int bd3_paged_attn(const void* q, const void* k_pages, const void* v_pages, void
   const int64_t bm = rows > kPagedMaxRows ? bd3::kPtBM : rows > 16 ? 32 : 16;
   const int bn = bm == bd3::kPtBM ? bd3::kPtBN : bd3::kPgBN;
   p.row_tiles = static_cast<int>((rows + bm - 1) / bm);
-  if (B * p.row_tiles > (1LL << 30)) return fail(BD3_ERR_UNSUPPORTED, "too many row tiles");
+  if (B * p.row_tiles > (1LL << 30) || (max_pages * page_size / bn + 16) * Hkv > (1LL << 30))
+    return fail(BD3_ERR_UNSUPPORTED, "too many row tiles");
   p.box = static_cast<int>(gcd64(page_size, bn));
   p.min_chunk = 1;
   CUtensorMap tk, tv;

@@ -22,6 +22,7 @@ namespace bd3 {
 
 constexpr int kPgBN = 64;                      // keys per tile
 constexpr int kPgThreads = 160;                // 4 consumer warps + 1 producer warp
+constexpr int kPgItemCost = 2;                 // an item's fixed cost in tiles
 constexpr uint32_t kPgTile = kPgBN * 128u;     // 64 keys x 128 B
 
 template <int kMB>
@@ -95,14 +96,14 @@ __global__ void __launch_bounds__(kPgThreads, 2)
   // the lengths, the new rows of the cache and the workspace come from the kernels before
   griddep_wait();
   griddep_launch_dependents();
-  PagedCursor cur = paged_chunk<kPgThreads, kRows, kPgBN>(p, scan);  // (its barriers cover the init)
+  PagedCursor cur = paged_chunk<kPgThreads, 1, kRows, kPgBN, kPgItemCost>(p, scan, 0);  // (its barriers cover the init)
   PagedItem it;
 
   if (warp == 4) {
     // ---------------- producer ----------------
     int J = 0;
     bool ok = true;
-    while (ok && paged_next<kRows, kPgBN>(p, cur, it)) {
+    while (ok && paged_next<kRows, kPgBN, kPgItemCost>(p, cur, it)) {
       ok = paged_stream<kPgBN>(
           p, it, J,
           [&](int j) {
@@ -129,7 +130,7 @@ __global__ void __launch_bounds__(kPgThreads, 2)
   float* s_l = s_m + 4 * kRows;
   int J = 0;
   bool ok = true;
-  while (paged_next<kRows, kPgBN>(p, cur, it)) {
+  while (paged_next<kRows, kPgBN, kPgItemCost>(p, cur, it)) {
     const int rows = it.s.qn * p.G, r0 = it.i * kRows;
     uint32_t qa[kMB][4][4];  // A fragments: m-block, k-step (16 of the 64 dims), regs
     int row_hi[kMB][2];

@@ -3,54 +3,64 @@
 // sequences. paged_sched.cuh has the layout, the visible keys and the distribution of work,
 // paged_attn.cuh the mathematics (the same, on 128-row tiles).
 //
-// One CTA per SM steps through its share of the work list, 128 x 128 score tiles, with TMEM,
-// barriers, the K/V ring and the double-buffered Q tile kept across items. The tensor cores
-// need 512 cycles a tile at D = 64 and the exponentials 1024 (16 a cycle and SM), so the
-// softmax bounds it: two warpgroups share a tile by key columns, each with its own running
-// max, sum and O accumulator in TMEM (no exchange per tile), merged once per item. S is
-// double-buffered, so the tensor cores work on tile j + 1 during the softmax of tile j.
-// Roles (320 threads):
-//   warps 0-3  softmax, key columns [0, 64) of every tile: thread t owns row t (TMEM lane t); at
-//              an item's end they merge the halves and write O, or the share's partial
-//   warps 4-7  softmax, key columns [64, 128)
-//   warp 8     producer: Q rows (token, head) by cp.async into the swizzled tile, K and V pieces
-//              page by page by TMA
-//   warp 9     TMEM owner and UMMA issuer: S = Q K^T (SS), then O_g += P_g V_g (P from TMEM)
-// TMEM columns: S0 [0,128), S1 [128,256), O_0 [256,320), O_1 [320,384); P_g (16-bit pairs)
-// overwrites the S columns that warpgroup g has read. O_g is rescaled only when a row's max
-// grows by more than 2^8 (log2 domain), voted per warp.
+// The tensor cores need 512 cycles for a 128 x 128 tile at D = 64 and the exponentials 1024 (16 a
+// cycle and SM), so the softmax bounds it, and within it the latency of its chain (TMEM load,
+// row max, exponentials, P store): one warpgroup alone leaves the exponential units idle for
+// most of a tile. So each SM runs two independent workers, each with its own chunk of the work
+// list, Q tile, K/V ring, TMEM columns and three roles, and nothing synchronises them: one's
+// exponentials fill the other's loads and waits. Per worker x (384 threads in all):
+//   warps 4x..4x+3  softmax: thread t owns row t (TMEM lane t) and all 128 columns of a tile; at a
+//                   share's end O / l to global memory, or the share's partial
+//   warp 8 + x      producer: Q rows (token, head) by cp.async into the swizzled tile, K and V
+//                   pieces page by page by TMA
+//   warp 10 + x     UMMA issuer (warp 10 owns the TMEM): S = Q K^T (SS), then O += P V (P from TMEM)
+// TMEM columns: S_x [128x, +128), P_x (16-bit pairs) [256 + 64x, +64), O_x [384 + 64x, +64). S_x is
+// released as soon as its rows are in registers, so the next S is computed during the
+// exponentials. O is rescaled only when a row's max grows by more than 2^8 (log2 domain),
+// voted per warp.
 #pragma once
 
-#include "attn_fwd.cuh"
+#include "attn_fwd_pair.cuh"
 #include "paged_attn.cuh"
 
 namespace bd3 {
 
 constexpr int kPtBM = 128, kPtBN = 128;
-constexpr int kPtStages = 4;
-constexpr int kPtThreads = 320;
+constexpr int kPtStages = 3;
+constexpr int kPtThreads = 384;
+constexpr int kPtItemCost = 2;     // an item's fixed cost in key tiles
 constexpr int kPtSlot = 128 * 66;  // floats of a partial: m[128], l[128], O[16][128] float4
 
 struct PtSmem {
-  static constexpr uint32_t kQ = 0;                             // [item parity]
-  static constexpr uint32_t kK = kQ + 2 * kTile16;
-  static constexpr uint32_t kV = kK + kPtStages * kTile16;
-  static constexpr uint32_t kBar = kV + kPtStages * kTile16;
-  // q_full[2], q_empty[2], k_full[S], v_full[S], kv_empty[S], s_full[2], p_full[2], o_done[2],
-  // o_free
-  static constexpr uint32_t kNumBars = 4 + 3 * kPtStages + 7;
-  static constexpr uint32_t kMerge = kBar + kNumBars * 8;       // [item parity] warpgroup 1's m, l
-  static constexpr uint32_t kScan = kMerge + 2 * 2 * 128 * 4;
-  static constexpr uint32_t kTmemSlot = kScan + ((sizeof(PagedScan) + 15) / 16) * 16;
-  static constexpr uint32_t kLast = kTmemSlot + 8;
-  static constexpr uint32_t kBytes = kTmemSlot + 16;
+  // per worker: Q, then K and V of each stage
+  static constexpr uint32_t kQ = 0, kK = kTile16, kV = kK + kPtStages * kTile16;
+  static constexpr uint32_t kWorker = kV + kPtStages * kTile16;
+  static constexpr uint32_t kBar = 2 * kWorker;
+  // per worker: q_full, q_empty, s_full, s_free, p_full, o_done, o_free, k_full[S], v_full[S],
+  // kv_empty[S]
+  static constexpr uint32_t kNumBars = 7 + 3 * kPtStages;
+  static constexpr uint32_t kScan = kBar + 2 * kNumBars * 8;
+  static constexpr uint32_t kTmemSlot = kScan + sizeof(PagedScan);
+  static constexpr uint32_t kLast = kTmemSlot + 8;  // [worker]
+  static constexpr uint32_t kBytes = kLast + 8;
   static constexpr uint32_t kAlloc = kBytes + 1024;
 };
+static_assert(PtSmem::kAlloc <= 227 * 1024, "shared memory of one CTA");
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
                "r"(live ? 16u : 0u)
                : "memory");
+}
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      " selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
 }
 
 template <bool kBF16>
@@ -61,39 +71,31 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + ((1024u - (raw_addr & 1023u)) & 1023u);
-  const uint32_t sbase = smem_u32(smem);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + PtSmem::kBar);
-  uint64_t* q_full = bars;
-  uint64_t* q_empty = bars + 2;
-  uint64_t* k_full = bars + 4;
-  uint64_t* v_full = k_full + kPtStages;
-  uint64_t* kv_empty = v_full + kPtStages;
-  uint64_t* s_full = kv_empty + kPtStages;  // [buffer]
-  uint64_t* p_full = s_full + 2;            // [warpgroup]
-  uint64_t* o_done = s_full + 4;            // [warpgroup]
-  uint64_t* o_free = s_full + 6;            // O_0 and O_1 of the item have been read
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + PtSmem::kTmemSlot);
-  int* last_flag = reinterpret_cast<int*>(smem + PtSmem::kLast);
   const int warp = static_cast<int>(warp_id());
   const int lane = static_cast<int>(lane_id());
+  const int x = warp < 8 ? warp >> 2 : warp & 1;  // this warp's worker
+  uint8_t* const wsm = smem + x * PtSmem::kWorker;
+  const uint32_t wbase = smem_u32(wsm);
+  uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + PtSmem::kBar) + x * PtSmem::kNumBars;
+  uint64_t* const q_full = bars;
+  uint64_t* const q_empty = bars + 1;
+  uint64_t* const s_full = bars + 2;
+  uint64_t* const s_free = bars + 3;
+  uint64_t* const p_full = bars + 4;
+  uint64_t* const o_done = bars + 5;
+  uint64_t* const o_free = bars + 6;
+  uint64_t* const k_full = bars + 7;
+  uint64_t* const v_full = k_full + kPtStages;
+  uint64_t* const kv_empty = v_full + kPtStages;
 
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&q_full[i], 1);
-      mbar_init(&q_empty[i], 1);
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 128);
-      mbar_init(&o_done[i], 1);
-    }
-    for (int s = 0; s < kPtStages; ++s) {
-      mbar_init(&k_full[s], 1);
-      mbar_init(&v_full[s], 1);
-      mbar_init(&kv_empty[s], 1);
-    }
-    mbar_init(o_free, 128);
+  if (threadIdx.x < 2) {
+    uint64_t* bb = reinterpret_cast<uint64_t*>(smem + PtSmem::kBar) + threadIdx.x * PtSmem::kNumBars;
+    for (int i = 0; i < static_cast<int>(PtSmem::kNumBars); ++i)
+      mbar_init(&bb[i], i == 3 || i == 4 || i == 6 ? 128 : 1);  // s_free, p_full, o_free
     fence_mbar_init();
   }
-  if (warp == 9) {
+  if (warp == 10) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
@@ -104,44 +106,51 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   tc_fence_before();
   griddep_wait();
   griddep_launch_dependents();
-  PagedCursor cur = paged_chunk<kPtThreads, kPtBM, kPtBN>(p, reinterpret_cast<PagedScan*>(smem + PtSmem::kScan));
+  PagedCursor cur = paged_chunk<kPtThreads, 2, kPtBM, kPtBN, kPtItemCost>(
+      p, reinterpret_cast<PagedScan*>(smem + PtSmem::kScan), x);
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   PagedItem it;
 
-  if (warp == 8) {
+  if (warp >= 8 && warp < 10) {
     // ---------------- producer ----------------
     bool ok = true;
     int J = 0;  // key tiles loaded so far
-    for (int n = 0; ok && paged_next<kPtBM, kPtBN>(p, cur, it); ++n) {
-      const int qb = n & 1;
-      if (n >= 2) ok = mbar_wait_warp(&q_empty[qb], ((n >> 1) - 1) & 1);
-      if (!ok) break;
-      const int rows = it.s.qn * p.G, r0 = it.i * kPtBM;
-      const uint32_t sq = sbase + PtSmem::kQ + qb * kTile16;
-#pragma unroll 4
-      for (int i = 0; i < 32; ++i) {
-        const int row = i * 4 + (lane >> 3), c = lane & 7;
-        const int r = r0 + row;
-        const bool live = r < rows;
-        const int t = live ? r / p.G : 0;
-        const uint16_t* src = reinterpret_cast<const uint16_t*>(p.q) + (it.s.q0 + t) * p.q_st +
-                              (it.h * p.G + (live ? r - t * p.G : 0)) * p.q_sh + c * 8;
-        cp_async16(sq + sw128_offset(row, c), src, live);
-      }
+    for (int n = 0; ok && paged_next<kPtBM, kPtBN, kPtItemCost>(p, cur, it); ++n) {
+      // Q: issued first for the first item, and for a later one after its first K/V tile (the Q
+      // tile is in use until the last S of the item before)
       bool q_sent = false;
+      auto load_q = [&]() {
+        if (n > 0 && !mbar_wait_warp(q_empty, (n - 1) & 1)) return false;
+        const int rows = it.s.qn * p.G, r0 = it.i * kPtBM;
+#pragma unroll 4
+        for (int i = 0; i < 32; ++i) {
+          const int row = i * 4 + (lane >> 3), c = lane & 7;
+          const int r = r0 + row;
+          const bool live = r < rows;
+          const int t = live ? r / p.G : 0;
+          const uint16_t* src = reinterpret_cast<const uint16_t*>(p.q) + (it.s.q0 + t) * p.q_st +
+                                (it.h * p.G + (live ? r - t * p.G : 0)) * p.q_sh + c * 8;
+          cp_async16(wbase + PtSmem::kQ + sw128_offset(row, c), src, live);
+        }
+        return true;
+      };
       auto send_q = [&]() {  // the rows are in shared memory: hand them to the tensor cores
         asm volatile("cp.async.wait_all;" ::: "memory");
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&q_full[qb]);
+        if (lane == 0) mbar_arrive(q_full);
         q_sent = true;
       };
       const int J0 = J;
-      ok = paged_stream<kPtBN>(
+      if (n == 0) ok = load_q();
+      ok = ok && paged_stream<kPtBN>(
           p, it, J,
           [&](int j) {
-            if (j == J0 + 1 && !q_sent) send_q();  // with the first K and V tile on their way
+            if (j == J0 + 1 && !q_sent) {
+              if (n > 0 && !load_q()) return false;
+              send_q();
+            }
             const int st = j % kPtStages;
             if (j >= kPtStages && !mbar_wait_warp(&kv_empty[st], ((j / kPtStages) - 1) & 1))
               return false;
@@ -154,77 +163,83 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           [&](int j, int piece, int page, int row) {
             const int st = j % kPtStages;
             const uint32_t off = st * kTile16 + piece * p.box * 128;
-            tma_load_4d(&tm_k, &k_full[st], smem + PtSmem::kK + off, 0, row, it.h, page);
-            tma_load_4d(&tm_v, &v_full[st], smem + PtSmem::kV + off, 0, row, it.h, page);
+            tma_load_4d(&tm_k, &k_full[st], wsm + PtSmem::kK + off, 0, row, it.h, page);
+            tma_load_4d(&tm_v, &v_full[st], wsm + PtSmem::kV + off, 0, row, it.h, page);
           });
-      if (!q_sent) send_q();
+      if (ok && !q_sent) {
+        if (n > 0) ok = load_q();
+        if (ok) send_q();
+      }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
     __syncwarp();
-  } else if (warp == 9) {
+  } else if (warp >= 10) {
     // ---------------- UMMA issuer ----------------
     if (elect_one()) {
       constexpr uint32_t idesc_qk = idesc_f16(128, 128, false, false, kBF16);
       constexpr uint32_t idesc_pv = idesc_f16(128, 64, false, true, kBF16);
-      bool ok = true;
-      // O_g += P_g V[64g, 64g+64) of key tile Jg, then release its K/V stage; the first one of
-      // item n overwrites O, after the previous item's epilogue has read it
-      auto issue_pv = [&](int Jg, bool first, int n) {
-        const int st = Jg % kPtStages;
-        ok = ok && mbar_wait(&v_full[st], (Jg / kPtStages) & 1);
-        if (ok && first && n > 0) ok = mbar_wait(o_free, (n - 1) & 1);
-        for (int g = 0; g < 2 && ok; ++g) {
-          ok = mbar_wait(&p_full[g], Jg & 1);
-          if (!ok) break;
-          tc_fence_after();
-          const uint64_t vdesc =
-              sw128_desc(sbase + PtSmem::kV + st * kTile16 + g * (kTile16 / 2), kTile16, 1024);
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            umma_ts(tmem + 256 + g * 64, tmem + (Jg & 1) * 128 + g * 64 + kk * 8,
-                    vdesc + ((kk * 2048) >> 4), idesc_pv, (!first || kk > 0) ? 1u : 0u);
-          umma_commit(&o_done[g]);
-        }
-        if (ok) umma_commit(&kv_empty[st]);
-      };
-      // S of a tile is issued before O += P V of the one before it, across items too
-      int J = 0, prev_J = -1, prev_n = 0;
-      bool prev_first = false;
-      for (int n = 0; ok && paged_next<kPtBM, kPtBN>(p, cur, it); ++n) {
-        const int qb = n & 1;
-        ok = mbar_wait(&q_full[qb], (n >> 1) & 1);
-        if (!ok) break;
+      const uint64_t qdesc = sw128_desc(wbase + PtSmem::kQ, 16, 1024);
+      bool ok = true, first = false, pending = false;
+      int J = 0, pn = 0;
+      // O += P V of tile J - 1, then release its K/V stage; the first one of item pn overwrites
+      // O, after the epilogue of the item before has read it
+      auto issue_pv = [&]() {
+        const int j = J - 1, st = j % kPtStages;
+        pending = false;
+        ok = ok && mbar_wait(&v_full[st], (j / kPtStages) & 1);
+        if (ok && first && pn > 0) ok = mbar_wait(o_free, (pn - 1) & 1);
+        ok = ok && mbar_wait(p_full, j & 1);
+        if (!ok) return;
         tc_fence_after();
-        const uint64_t qdesc = sw128_desc(sbase + PtSmem::kQ + qb * kTile16, 16, 1024);
-        for (int t = it.t0; ok && t < it.t1; ++t, ++J) {
+        const uint64_t vdesc = sw128_desc(wbase + PtSmem::kV + st * kTile16, kTile16, 1024);
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)
+          umma_ts(tmem + 384 + x * 64, tmem + 256 + x * 64 + kk * 8, vdesc + ((kk * 2048) >> 4),
+                  idesc_pv, (!first || kk > 0) ? 1u : 0u);
+        umma_commit(o_done);
+        umma_commit(&kv_empty[st]);
+      };
+      for (int n = 0; ok && paged_next<kPtBM, kPtBN, kPtItemCost>(p, cur, it); ++n) {
+        // S of a tile goes before O += P V of the one before it, so that it is ready when that
+        // tile's softmax ends; at an item's start only if its Q and K are there already
+        if (pending && !(mbar_test(q_full, n & 1) &&
+                         mbar_test(&k_full[J % kPtStages], (J / kPtStages) & 1)))
+          issue_pv();
+        ok = ok && mbar_wait(q_full, n & 1);
+        for (int t = it.t0; ok && t < it.t1; ++t) {
           const int st = J % kPtStages;
           ok = mbar_wait(&k_full[st], (J / kPtStages) & 1);
+          if (ok && J > 0) ok = mbar_wait(s_free, (J - 1) & 1);  // S is in registers
           if (!ok) break;
           tc_fence_after();
-          const uint64_t kdesc = sw128_desc(sbase + PtSmem::kK + st * kTile16, 16, 1024);
+          const uint64_t kdesc = sw128_desc(wbase + PtSmem::kK + st * kTile16, 16, 1024);
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
-            umma_ss(tmem + (J & 1) * 128, qdesc + ((kk * 32) >> 4), kdesc + ((kk * 32) >> 4),
-                    idesc_qk, kk > 0 ? 1u : 0u);
-          umma_commit(&s_full[J & 1]);
-          if (t == it.t1 - 1) umma_commit(&q_empty[qb]);
-          if (prev_J >= 0) issue_pv(prev_J, prev_first, prev_n);
-          prev_J = J;
-          prev_first = t == it.t0;
-          prev_n = n;
+            umma_ss(tmem + x * 128, qdesc + ((kk * 32) >> 4), kdesc + ((kk * 32) >> 4), idesc_qk,
+                    kk > 0 ? 1u : 0u);
+          umma_commit(s_full);
+          if (t == it.t1 - 1) umma_commit(q_empty);
+          if (pending) issue_pv();
+          ++J;
+          pending = true;
+          first = t == it.t0;
+          pn = n;
         }
       }
-      if (ok && prev_J >= 0) issue_pv(prev_J, prev_first, prev_n);
+      if (ok && pending) issue_pv();
     }
     __syncwarp();
   } else {
-    // ---------------- softmax: warpgroup g owns key columns [64g, 64g+64) ----------------
-    const int g = warp >> 2;
+    // ---------------- softmax ----------------
     const int row = threadIdx.x & 127;
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t tO = tmem + lane_base + 256 + g * 64;
+    const uint32_t tS = tmem + lane_base + x * 128;
+    const uint32_t tP = tmem + lane_base + 256 + x * 64;
+    const uint32_t tO = tmem + lane_base + 384 + x * 64;
+    int* const last_flag = reinterpret_cast<int*>(smem + PtSmem::kLast) + x;
     bool ok = true;
     int J = 0;  // key tiles consumed so far
-    for (int n = 0; paged_next<kPtBM, kPtBN>(p, cur, it); ++n) {
+    while (paged_next<kPtBM, kPtBN, kPtItemCost>(p, cur, it)) {
       const int rows = it.s.qn * p.G, r = it.i * kPtBM + row;
       const bool live = r < rows;
       const int tok = live ? r / p.G : 0;
@@ -232,43 +247,48 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       const int full_all = paged_hi(p, it.s, it.i * kPtBM / p.G);  // seen by every row
       const bool dead = !__any_sync(0xffffffffu, live);  // a warp without rows computes nothing
       float m_run = -INFINITY, l_run = 0.f;
-      int Jg = J;
-      for (int t = it.t0; t < it.t1; ++t, ++Jg) {
-        const int s = t * kPtBN, b = Jg & 1;
-        ok = mbar_wait_warp(&s_full[b], (Jg >> 1) & 1);
+      for (int t = it.t0; t < it.t1; ++t, ++J) {
+        const int s = t * kPtBN;
+        ok = mbar_wait_warp(s_full, J & 1);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t tS = tmem + lane_base + b * 128 + g * 64;
-        const bool masked = s + kPtBN > full_all;
-        const int hi = row_hi - s - g * 64;  // this row's visible columns of the 64: [0, hi)
-        const bool skip = dead || (masked && __all_sync(0xffffffffu, hi <= 0));
-        float alpha = 1.f, sum = 0.f;
-        bool rescale = false;
-        if (skip) {
-          uint32_t zero[32];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) zero[i] = 0u;
-          if (!dead) tmem_st32(tS, zero);  // (the O rows of a dead warp are not read)
+        if (dead) {  // (the P and O rows of a dead warp are never read)
+          tc_fence_before();
+          mbar_arrive(s_free);
+          // as the other warps do: an arrival for this P before the last one is complete would
+          // count for the last one
+          if (t > it.t0) ok = mbar_wait_warp(o_done, (J - 1) & 1);
+          if (!ok) break;
         } else {
-          float x[64];
+          const bool masked = s + kPtBN > full_all;
+          const int hi = masked ? row_hi - s : kPtBN;  // this row sees columns [0, hi)
+          uint32_t vis = 0;  // 32-column chunks that some row of the warp sees
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (__any_sync(0xffffffffu, hi > 32 * c)) vis |= 1u << c;
+          float xs[128];
           {
-            uint32_t u[2][32];
-            tmem_ld32_async(tS, u[0]);
-            tmem_ld32_async(tS + 32, u[1]);
+            uint32_t u[4][32];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tmem_ld32_async(tS + c * 32, u[c]);
             tmem_ld_wait();
 #pragma unroll
-            for (int c2 = 0; c2 < 2; ++c2) {
-              reg_fence(u[c2]);
+            for (int c = 0; c < 4; ++c) {
+              reg_fence(u[c]);
 #pragma unroll
-              for (int i = 0; i < 32; ++i) x[c2 * 32 + i] = __uint_as_float(u[c2][i]);
+              for (int k = 0; k < 32; ++k) xs[c * 32 + k] = __uint_as_float(u[c][k]);
             }
           }
-          if (masked) {
-#pragma unroll
-            for (int c = 0; c < 64; ++c)
-              if (c >= hi) x[c] = -INFINITY;
-          }
-          const float m_new = fmaxf(m_run, max64(x) * p.scale_log2);
+          tc_fence_before();
+          mbar_arrive(s_free);  // S is in registers: the next one may be computed
+          const float mx = max3(chunk_max<0>(xs, vis, masked, 0, hi),
+                                chunk_max<1>(xs, vis, masked, 0, hi),
+                                fmaxf(chunk_max<2>(xs, vis, masked, 0, hi),
+                                      chunk_max<3>(xs, vis, masked, 0, hi))) *
+                           p.scale_log2;
+          float alpha = 1.f;
+          bool rescale = false;
+          const float m_new = fmaxf(m_run, mx);
           if (m_new - m_run > kRescaleLog2) {  // false for NaN (-inf - -inf)
             alpha = ex2(m_run - m_new);        // 0 when m_run = -inf
             rescale = t > it.t0;
@@ -279,95 +299,82 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           const float2 nm2 = make_float2(-m_use, -m_use);
           float2 acc[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f),
                            make_float2(0.f, 0.f)};
-          uint32_t pk[32];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float2 z = __ffma2_rn(make_float2(x[2 * i], x[2 * i + 1]), sc2, nm2);
-            const float2 e = make_float2(ex2(z.x), ex2(z.y));
-            acc[i & 3] = __fadd2_rn(acc[i & 3], e);
-            pk[i] = pack2<kBF16>(e.x, e.y);
+          for (int c = 0; c < 4; ++c) {
+            uint32_t pk[16];
+            if (vis & (1u << c)) {
+#pragma unroll
+              for (int k = 0; k < 16; ++k) {
+                const int gi = c * 16 + k;  // column pair of the row
+                const float2 z = __ffma2_rn(make_float2(xs[2 * gi], xs[2 * gi + 1]), sc2, nm2);
+                const float2 e = make_float2(ex2(z.x), ex2(z.y));
+                acc[k & 3] = __fadd2_rn(acc[k & 3], e);
+                pk[k] = pack2<kBF16>(e.x, e.y);
+              }
+            } else {
+#pragma unroll
+              for (int k = 0; k < 16; ++k) pk[k] = 0u;
+            }
+            if (c == 0 && t > it.t0) {
+              ok = mbar_wait_warp(o_done, (J - 1) & 1);  // the P of the tile before is used up
+              tc_fence_after();
+            }
+            tmem_st16(tP + c * 16, pk);
           }
+          if (!ok) break;
           const float2 a01 = __fadd2_rn(__fadd2_rn(acc[0], acc[1]), __fadd2_rn(acc[2], acc[3]));
-          sum = a01.x + a01.y;
-          tmem_st32(tS, pk);
-        }
-        l_run = l_run * alpha + sum;
-        tmem_st_wait();
-        if (it.hi - s < kPtBN) {
-          // Rows of V past the visible keys hold what the page holds there, NaN included, and
-          // P = 0 does not cancel that: zero this warpgroup's half of them before P V.
-          const int st = Jg % kPtStages;
-          ok = mbar_wait_warp(&v_full[st], (Jg / kPtStages) & 1);
-          if (!ok) break;
-          const int key = g * 64 + (row >> 1);
-          if (key >= it.hi - s) {
-            uint8_t* v = smem + PtSmem::kV + st * kTile16 + key * 128 + (row & 1) * 64;
+          l_run = l_run * alpha + (a01.x + a01.y);
+          if (__any_sync(0xffffffffu, rescale)) {  // rows that do not need it multiply by 1
+            uint32_t u[2][32];
+            tmem_ld32_async(tO, u[0]);
+            tmem_ld32_async(tO + 32, u[1]);
+            tmem_ld_wait();
 #pragma unroll
-            for (int c = 0; c < 4; ++c) *reinterpret_cast<uint4*>(v + 16 * c) = make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async_smem();
-        }
-        if (t > it.t0) {
-          ok = mbar_wait_warp(&o_done[g], (Jg - 1) & 1);  // O_g += P_g V of the tile before
-          if (!ok) break;
-          tc_fence_after();
-        }
-        if (__any_sync(0xffffffffu, rescale)) {  // rows that do not need it multiply by 1
-          uint32_t u[2][32];
-          tmem_ld32_async(tO, u[0]);
-          tmem_ld32_async(tO + 32, u[1]);
-          tmem_ld_wait();
+            for (int c2 = 0; c2 < 2; ++c2) {
+              reg_fence(u[c2]);
 #pragma unroll
-          for (int c2 = 0; c2 < 2; ++c2) {
-            reg_fence(u[c2]);
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              u[c2][i] = __float_as_uint(__uint_as_float(u[c2][i]) * alpha);
-            tmem_st32(tO + c2 * 32, u[c2]);
+              for (int k = 0; k < 32; ++k)
+                u[c2][k] = __float_as_uint(__uint_as_float(u[c2][k]) * alpha);
+              tmem_st32(tO + c2 * 32, u[c2]);
+            }
           }
           tmem_st_wait();
         }
+        if (it.hi - s < kPtBN) {
+          // Rows of V past the visible keys hold what the page holds there, NaN included, and
+          // P = 0 does not cancel that: zero them before P V.
+          const int st = J % kPtStages;
+          ok = mbar_wait_warp(&v_full[st], (J / kPtStages) & 1);
+          if (!ok) break;
+          if (row >= it.hi - s) {
+            uint8_t* v = wsm + PtSmem::kV + st * kTile16 + row * 128;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(v + 16 * c) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+        }
         tc_fence_before();
-        mbar_arrive(&p_full[g]);
+        mbar_arrive(p_full);
       }
-      // ---- the item's end: merge the halves; write O, or this share's partial ----
-      if (ok) ok = mbar_wait_warp(&o_done[g], (Jg - 1) & 1);
-      J = Jg;
-      float* merge_m = reinterpret_cast<float*>(smem + PtSmem::kMerge) + (n & 1) * 256;
-      float* merge_l = merge_m + 128;
-      if (g == 1) {
-        merge_m[row] = m_run;
-        merge_l[row] = l_run;
+      // ---- the share's end: the last O += P V has landed; O / l, or the share's partial ----
+      if (ok) ok = mbar_wait_warp(o_done, (J - 1) & 1);
+      if (!bar_and(1 + x, 128, ok)) break;
+      tc_fence_after();
+      float o[64], L = l_run, M = m_run;
+      {
+        uint32_t u[2][32];
+        tmem_ld32_async(tO, u[0]);
+        tmem_ld32_async(tO + 32, u[1]);
+        tmem_ld_wait();
+#pragma unroll
+        for (int c2 = 0; c2 < 2; ++c2) {
+          reg_fence(u[c2]);
+#pragma unroll
+          for (int k = 0; k < 32; ++k) o[c2 * 32 + k] = __uint_as_float(u[c2][k]);
+        }
       }
       tc_fence_before();
-      if (!bar_and(1, 256, ok)) break;
-      tc_fence_after();
-      if (g == 1) continue;
-      const float m1 = merge_m[row], l1 = merge_l[row];
-      float M = fmaxf(m_run, m1);
-      float Mu = M == -INFINITY ? 0.f : M;
-      const float w0 = ex2(m_run - Mu), w1 = ex2(m1 - Mu);  // 0 for a half that saw no key
-      float L = l_run * w0 + l1 * w1;
-      float o[64];
-      {
-        uint32_t u0[2][32], u1[2][32];
-#pragma unroll
-        for (int c2 = 0; c2 < 2; ++c2) {
-          tmem_ld32_async(tmem + lane_base + 256 + c2 * 32, u0[c2]);
-          tmem_ld32_async(tmem + lane_base + 320 + c2 * 32, u1[c2]);
-        }
-        tmem_ld_wait();
-        tc_fence_before();
-        mbar_arrive(o_free);  // the next item may overwrite O_0 and O_1
-#pragma unroll
-        for (int c2 = 0; c2 < 2; ++c2) {
-          reg_fence(u0[c2]);
-          reg_fence(u1[c2]);
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            o[c2 * 32 + i] = __uint_as_float(u0[c2][i]) * w0 + __uint_as_float(u1[c2][i]) * w1;
-        }
-      }
+      mbar_arrive(o_free);  // O is in registers: the next item may overwrite it
       if (it.parts > 1) {
         float* slot = p.partials + static_cast<long long>(it.slot) * kPtSlot;
         if (live) {
@@ -378,18 +385,17 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           for (int c = 0; c < 16; ++c)
             dst[c * 128] = make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
         }
-        // the share that finishes last merges the item's partials, in CTA order
-        asm volatile("bar.sync 2, 128;" ::: "memory");
-        if (threadIdx.x == 0) {
+        // the share that finishes last merges the item's partials, in list order
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + x) : "memory");
+        if (row == 0) {
           __threadfence();
           const int before = atomicAdd(&p.counters[it.slot0], 1);
           *last_flag = before == it.parts - 1;
           if (before == it.parts - 1) p.counters[it.slot0] = 0;
           __threadfence();
         }
-        asm volatile("bar.sync 2, 128;" ::: "memory");
-        const bool last = *last_flag != 0;
-        if (!last) continue;
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + x) : "memory");
+        if (*last_flag == 0) continue;
         M = -INFINITY;
         L = 0.f;
 #pragma unroll
@@ -411,7 +417,6 @@ __global__ void __launch_bounds__(kPtThreads, 1)
             o[4 * c + 3] = o[4 * c + 3] * a + v.w * w;
           }
         }
-        Mu = M == -INFINITY ? 0.f : M;
       }
       if (live) {
         const float inv = L == 0.f ? 0.f : 1.f / L;  // L = 0: a row without keys
@@ -426,13 +431,14 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         }
         if (p.lse != nullptr)
           p.lse[static_cast<long long>(it.s.q0 + tok) * (p.Hkv * p.G) + hq] =
-              L == 0.f ? -INFINITY : (Mu + log2f(L)) * 0.69314718055994530942f;
+              L == 0.f ? -INFINITY
+                       : ((M == -INFINITY ? 0.f : M) + log2f(L)) * 0.69314718055994530942f;
       }
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == 10) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }

@@ -7,17 +7,19 @@
 // KV head's keys are read once for all of them.
 //
 // Work is a list of items (sequence b, row tile i, KV head h), each with n(b, i) key tiles, laid
-// end to end in that order; W is its length in key tiles. The lengths live on the device (a
-// captured launch serves every step of a growing batch), so each CTA computes the prefix sums
-// of n itself: the threads sum n * Hkv over their share of the (b, i) pairs, a block scan gives
-// every share's start. CTA c then takes tiles [c * chunk, (c + 1) * chunk) of the list,
-// chunk = max(ceil(W / CTAs), a minimum): the same number of tiles for every CTA whatever
-// the mix of lengths, so one 64K-token sequence among short ones does not set the time.
-// An item cut by chunk borders leaves one partial (m, l, unnormalised O) per CTA in the
-// workspace; the CTA that finishes last (an atomic count per cut item) merges the partials in
-// CTA order, so the sum's order does not depend on timing. Nothing waits for another CTA. The
-// counts are zero before the first call (the caller's zeroed workspace) and the merging CTA
-// sets its count back to zero, so calls in stream order share one workspace.
+// end to end in that order; an item also counts kItemCost tiles for what it costs whatever its
+// length (finding it, its Q rows, its epilogue). W is the list's length. The lengths live on
+// the device (a captured launch serves every step of a growing batch), so each CTA computes
+// the prefix sums itself: the threads add up their share of the (b, i) pairs, a block scan
+// gives every share's start. Worker w (a CTA, or one of its independent halves) then takes
+// [w * chunk, (w + 1) * chunk) of the list, chunk = max(ceil(W / workers), a minimum): the
+// same work for every worker whatever the mix of lengths, so one 64K-token sequence among
+// short ones does not set the time.
+// An item cut by chunk borders leaves one partial (m, l, unnormalised O) per worker in the
+// workspace; the worker that finishes last (an atomic count per cut item) merges the partials
+// in list order, so the order of the sums does not depend on timing. Nothing waits for another
+// worker. The counts are zero before the first call (the caller's zeroed workspace) and the
+// merging worker sets its count back to zero, so calls in stream order share one workspace.
 #pragma once
 
 #include "common.cuh"
@@ -34,8 +36,8 @@ struct PagedParams {
   long long pt_stride;
   const int* kv_lens;         // (B)
   const int* cu_q;            // (B + 1)
-  int* counters;              // 2 per CTA, zero between calls
-  float* partials;            // 2 slots per CTA of (m, l, O) of a row tile
+  int* counters;              // 2 per worker, zero between calls
+  float* partials;            // 2 slots per worker of (m, l, O) of a row tile
   int B, Hkv, G, total_q, max_q;
   int num_pages, page_size, max_pages;
   int box;                    // rows of one TMA piece: divides the page size and the key tile
@@ -84,26 +86,27 @@ __device__ __forceinline__ int paged_tiles(const PagedParams& p, const PagedSeq&
   return hi > kBN ? (hi - 1) / kBN + 1 : 1;
 }
 
-// One CTA's share of an item.
+// One worker's share of an item.
 struct PagedItem {
   PagedSeq s;
   int b, i, h;
   int hi;         // exclusive end of the keys that any row of the item sees
   int t0, t1;     // key tiles of this share
-  int parts;      // CTAs that share the item; 1: this one alone
+  int parts;      // workers that share the item; 1: this one alone
   int slot;       // this share's partial
   int slot0;      // the first share's partial, and the item's count
-  int cta0;       // the first share's CTA
+  int w0;         // the first share's worker
 };
 
 struct PagedCursor {
+  int w;                      // this worker
   int b, i;
-  long long base;             // list position of the pair (b, i)'s first tile
+  long long base;             // list position of the pair (b, i)
   long long pos, lo, end, chunk;
 };
 
-// The next share of this CTA's chunk; false at its end.
-template <int kBM, int kBN>
+// The next share of this worker's chunk; false at its end.
+template <int kBM, int kBN, int kItemCost>
 __device__ __forceinline__ bool paged_next(const PagedParams& p, PagedCursor& c, PagedItem& it) {
   while (c.pos < c.end && c.b < p.B) {
     it.s = paged_seq(p, c.b);
@@ -113,7 +116,8 @@ __device__ __forceinline__ bool paged_next(const PagedParams& p, PagedCursor& c,
       c.i = 0;
       continue;
     }
-    const long long w = static_cast<long long>(n) * p.Hkv;
+    const int cost = n + kItemCost;
+    const long long w = static_cast<long long>(cost) * p.Hkv;
     if (c.pos >= c.base + w) {
       c.base += w;
       if (++c.i == p.row_tiles) {
@@ -124,47 +128,51 @@ __device__ __forceinline__ bool paged_next(const PagedParams& p, PagedCursor& c,
     }
     it.b = c.b;
     it.i = c.i;
-    it.h = static_cast<int>((c.pos - c.base) / n);
-    const long long start = c.base + static_cast<long long>(it.h) * n;  // the item's first tile
-    it.t0 = static_cast<int>(c.pos - start);
-    const long long left = c.end - c.pos;
-    it.t1 = left < n - it.t0 ? it.t0 + static_cast<int>(left) : n;
-    const long long c0 = start / c.chunk, c1 = (start + n - 1) / c.chunk;
-    it.cta0 = static_cast<int>(c0);
-    it.parts = static_cast<int>(c1 - c0) + 1;
-    it.slot0 = 2 * it.cta0 + (start == c0 * c.chunk ? 0 : 1);
-    it.slot = 2 * static_cast<int>(blockIdx.x) + (c.pos == c.lo ? 0 : 1);
-    c.pos += it.t1 - it.t0;
+    it.h = static_cast<int>(c.pos - c.base) / cost;  // (the host bounds cost * Hkv)
+    const long long first = c.base + static_cast<long long>(it.h) * cost + kItemCost;  // tile 0
+    const long long stop = first + n < c.end ? first + n : c.end;
+    const long long from = c.pos > first ? c.pos : first;
+    c.pos = stop > c.pos ? stop : c.end;
+    if (stop <= first) continue;  // only the item's fixed cost falls into this chunk
+    it.t0 = static_cast<int>(from - first);
+    it.t1 = static_cast<int>(stop - first);
+    const long long w0 = first / c.chunk, w1 = (first + n - 1) / c.chunk;
+    it.w0 = static_cast<int>(w0);
+    it.parts = static_cast<int>(w1 - w0) + 1;
+    it.slot0 = 2 * it.w0 + (first == w0 * c.chunk ? 0 : 1);
+    it.slot = 2 * c.w + (from == c.lo ? 0 : 1);
     return true;
   }
   return false;
 }
 // Partial slot of share j of an item.
 __device__ __forceinline__ int paged_part_slot(const PagedItem& it, int j) {
-  return j == 0 ? it.slot0 : 2 * (it.cta0 + j);
+  return j == 0 ? it.slot0 : 2 * (it.w0 + j);
 }
 
 struct PagedScan {
-  long long warp_sum[32];
-  long long base;
-  int b, i;
+  long long warp_sum[16];
+  long long base[2];
+  int b[2], i[2];
 };
 
-// This CTA's chunk of the list, found by all kThreads threads; ends with a barrier. The chunk
-// is empty (pos == end) for a CTA past the list.
-template <int kThreads, int kBM, int kBN>
-__device__ __forceinline__ PagedCursor paged_chunk(const PagedParams& p, PagedScan* sc) {
+// The chunk of worker kWorkers * blockIdx.x + x, found by all kThreads threads of the CTA for all
+// its workers at once; ends with a barrier. The chunk is empty for a worker past the list.
+template <int kThreads, int kWorkers, int kBM, int kBN, int kItemCost>
+__device__ __forceinline__ PagedCursor paged_chunk(const PagedParams& p, PagedScan* sc, int x) {
+  static_assert(kThreads <= 512 && kWorkers <= 2, "PagedScan");
   const int pairs = p.B * p.row_tiles;
   const int per = cdiv(pairs, kThreads);
   const int e0 = imin(static_cast<int>(threadIdx.x) * per, pairs), e1 = imin(e0 + per, pairs);
-  auto tiles = [&](int e) -> long long {
-    const PagedSeq s = paged_seq(p, e / p.row_tiles);
+  auto cost = [&](int e, int b) -> long long {
+    const PagedSeq s = paged_seq(p, b);
     if (s.bad && blockIdx.x == 0) atomicOr(&g_bd3_status, kStatusBadLaunch);
     int hi;
-    return static_cast<long long>(paged_tiles<kBM, kBN>(p, s, e % p.row_tiles, &hi)) * p.Hkv;
+    const int n = paged_tiles<kBM, kBN>(p, s, e - b * p.row_tiles, &hi);
+    return n == 0 ? 0 : static_cast<long long>(n + kItemCost) * p.Hkv;
   };
   long long mine = 0;
-  for (int e = e0; e < e1; ++e) mine += tiles(e);
+  for (int e = e0; e < e1; ++e) mine += cost(e, e / p.row_tiles);
   const int lane = static_cast<int>(lane_id()), w = static_cast<int>(threadIdx.x) >> 5;
   long long incl = mine;
 #pragma unroll
@@ -180,30 +188,36 @@ __device__ __forceinline__ PagedCursor paged_chunk(const PagedParams& p, PagedSc
     if (k == w) before = total;
     total += sc->warp_sum[k];
   }
+  const long long workers = static_cast<long long>(gridDim.x) * kWorkers;
   PagedCursor c;
-  c.chunk = (total + gridDim.x - 1) / gridDim.x;
+  c.chunk = (total + workers - 1) / workers;
   if (c.chunk < p.min_chunk) c.chunk = p.min_chunk;
-  c.lo = c.chunk * blockIdx.x;
-  c.end = c.lo + c.chunk < total ? c.lo + c.chunk : total;
-  c.pos = c.lo < c.end ? c.lo : c.end;
-  long long at = before + incl - mine;
-  if (c.lo >= at && c.lo < at + mine) {  // this thread's share holds the chunk's start
-    for (int e = e0; e < e1; ++e) {
-      const long long n = tiles(e);
-      if (c.lo < at + n) {
-        sc->base = at;
-        sc->b = e / p.row_tiles;
-        sc->i = e % p.row_tiles;
-        break;
+#pragma unroll
+  for (int k = 0; k < kWorkers; ++k) {
+    const long long lo = c.chunk * (static_cast<long long>(blockIdx.x) * kWorkers + k);
+    long long at = before + incl - mine;
+    if (lo >= at && lo < at + mine) {  // this thread's share holds the chunk's start
+      for (int e = e0; e < e1; ++e) {
+        const int b = e / p.row_tiles;
+        const long long n = cost(e, b);
+        if (lo < at + n) {
+          sc->base[k] = at;
+          sc->b[k] = b;
+          sc->i[k] = e - b * p.row_tiles;
+          break;
+        }
+        at += n;
       }
-      at += n;
     }
   }
   __syncthreads();
-  c.base = sc->base;
-  c.b = sc->b;
-  c.i = sc->i;
-  if (c.pos >= c.end) c.b = p.B;
+  c.w = static_cast<int>(blockIdx.x) * kWorkers + x;
+  c.lo = c.chunk * c.w;
+  c.end = c.lo + c.chunk < total ? c.lo + c.chunk : total;
+  c.pos = c.lo;
+  c.base = sc->base[x];
+  c.b = c.lo < c.end ? sc->b[x] : p.B;
+  c.i = sc->i[x];
   return c;
 }
 
@@ -229,9 +243,9 @@ __device__ __forceinline__ int paged_lookup(const PagedParams& p, const PagedIte
   return id;
 }
 
-// Stream K and V pieces of the item's key tiles [t0, t1) into a ring, whole warp: stage(J) waits
-// for ring slot J and returns the K destination (0: gave up), V follows at `v_off`.
-// (The two kernels differ in their rings, so they pass the waits and barriers in.)
+// Stream K and V pieces of the item's key tiles [t0, t1) into a ring, whole warp: wait(j) waits
+// for the ring slot of tile j (false: gave up) and announces its bytes, issue(j, piece, page,
+// row) loads one piece. J counts the tiles of all items.
 template <int kBN, typename Wait, typename Issue>
 __device__ __forceinline__ bool paged_stream(const PagedParams& p, const PagedItem& it, int& J,
                                              Wait&& wait, Issue&& issue) {

@@ -60,7 +60,7 @@ def run(dev, lens, block_size, **kw):
                               dev["kv_lens"], dev["cu_q"], max(n for n, _ in lens), block_size, **kw)
 
 
-def check(d, out, lse, block_size, scale=None):
+def check(d, out, lse, block_size, scale=None, part=slice(None)):
     dt = d["q"].dtype
     ref, ref_lse, mag = op.paged_attention(d["q"], d["k_pages"], d["v_pages"], d["page_table"],
                                            d["kv_lens"], d["cu_q"], block_size, scale)
@@ -69,8 +69,8 @@ def check(d, out, lse, block_size, scale=None):
     tol = 1.1 * (out_u * ref.abs() + U[dt] * mag) + 1e-6
     if dt == torch.float16:
         tol = tol + int(d["kv_lens"].max()) * 2.0 ** -25 * 5
-    bad = (o - ref).abs() > tol
-    assert torch.isfinite(o).all() and not bad.any(), \
+    bad = ((o - ref).abs() > tol)[part]
+    assert torch.isfinite(o[part]).all() and not bad.any(), \
         f"{int(bad.sum())} of {bad.numel()} off, worst {(o - ref).abs().max():.3e}"
     if lse is not None:
         got = lse.cpu().double()
@@ -268,13 +268,15 @@ def test_bad_lengths_and_pages_are_cut_and_reported(rows):
         o = run(bad, lens, 16, workspace=ws)
         torch.cuda.synchronize()
         assert ops.device_status() == 2, (name, value)
-        assert torch.equal(o[rows:], ref[rows:])
+        # (another length of the first sequence moves the borders between the shares: not the
+        # same bits)
+        check(d, o, None, 16, part=slice(rows, None))
     bad = {k: v.clone() for k, v in dev.items()}
     bad["cu_q"][2] = 10 ** 8
     o = run(bad, lens, 16, workspace=ws)
     torch.cuda.synchronize()
     assert ops.device_status() == 2
-    assert torch.equal(o[:rows], ref[:rows])
+    check(d, o, None, 16, part=slice(0, rows))
     assert torch.equal(run(dev, lens, 16, workspace=ws), ref)  # the workspace is as it was
 
 
