@@ -20,7 +20,7 @@
 // voted per warp.
 #pragma once
 
-#include "attn_fwd_pair.cuh"
+#include "attn_fwd.cuh"
 #include "paged_attn.cuh"
 
 namespace bd3 {
@@ -51,6 +51,18 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool l
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
                "r"(live ? 16u : 0u)
                : "memory");
+}
+// Max over 32 floats as a tree of three-input maxes.
+__device__ __forceinline__ float max32(const uint32_t (&u)[32]) {
+  float a[11], b[4];
+#pragma unroll
+  for (int i = 0; i < 10; ++i)
+    a[i] = max3(__uint_as_float(u[3 * i]), __uint_as_float(u[3 * i + 1]), __uint_as_float(u[3 * i + 2]));
+  a[10] = fmaxf(__uint_as_float(u[30]), __uint_as_float(u[31]));
+#pragma unroll
+  for (int i = 0; i < 3; ++i) b[i] = max3(a[3 * i], a[3 * i + 1], a[3 * i + 2]);
+  b[3] = fmaxf(a[9], a[10]);
+  return max3(b[0], b[1], fmaxf(b[2], b[3]));
 }
 __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
@@ -266,47 +278,64 @@ __global__ void __launch_bounds__(kPtThreads, 1)
 #pragma unroll
           for (int c = 0; c < 4; ++c)
             if (__any_sync(0xffffffffu, hi > 32 * c)) vis |= 1u << c;
-          float xs[128];
-          {
-            uint32_t u[4][32];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_ld32_async(tS + c * 32, u[c]);
-            tmem_ld_wait();
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              reg_fence(u[c]);
-#pragma unroll
-              for (int k = 0; k < 32; ++k) xs[c * 32 + k] = __uint_as_float(u[c][k]);
-            }
-          }
-          tc_fence_before();
-          mbar_arrive(s_free);  // S is in registers: the next one may be computed
-          const float mx = max3(chunk_max<0>(xs, vis, masked, 0, hi),
-                                chunk_max<1>(xs, vis, masked, 0, hi),
-                                fmaxf(chunk_max<2>(xs, vis, masked, 0, hi),
-                                      chunk_max<3>(xs, vis, masked, 0, hi))) *
-                           p.scale_log2;
-          float alpha = 1.f;
-          bool rescale = false;
-          const float m_new = fmaxf(m_run, mx);
-          if (m_new - m_run > kRescaleLog2) {  // false for NaN (-inf - -inf)
-            alpha = ex2(m_run - m_new);        // 0 when m_run = -inf
-            rescale = t > it.t0;
-            m_run = m_new;
-          }
-          const float m_use = m_run == -INFINITY ? 0.f : m_run;
-          const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
-          const float2 nm2 = make_float2(-m_use, -m_use);
+          // 32 columns at a time, the next ones on their way from TMEM: P = 2^(x scale - m) with the
+          // m of the chunks before, unless a row's max is more than 2^8 above it (as in an
+          // item's first chunk); then m is raised and what was summed or stored under the old
+          // one is scaled down.
           float2 acc[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f),
                            make_float2(0.f, 0.f)};
+          float alpha = 1.f;
+          bool rescale = false;  // the same for all lanes
+          uint32_t u[2][32];
+          tmem_ld32_async(tS, u[0]);
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
+            uint32_t(&uc)[32] = u[c & 1];
+            tmem_ld_wait();
+            reg_fence(uc);
+            if (c < 3) {
+              tmem_ld32_async(tS + 32 * (c + 1), u[(c + 1) & 1]);
+            } else {
+              tc_fence_before();
+              mbar_arrive(s_free);  // S is in registers: the next one may be computed
+            }
             uint32_t pk[16];
             if (vis & (1u << c)) {
+              if (masked) {
+#pragma unroll
+                for (int k = 0; k < 32; ++k)
+                  if (32 * c + k >= hi) uc[k] = 0xFF800000u;  // -inf
+              }
+              const float mx = max32(uc) * p.scale_log2;
+              const bool up = mx - m_run > kRescaleLog2;  // false for NaN (-inf - -inf)
+              if (__any_sync(0xffffffffu, up)) {
+                const float f = up ? ex2(m_run - mx) : 1.f;  // 0 when m_run = -inf
+                if (up) m_run = mx;
+                alpha *= f;
+                l_run *= f;
+                rescale = true;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[i] = __fmul2_rn(acc[i], make_float2(f, f));
+                tmem_st_wait();
+#pragma unroll
+                for (int d = 0; d < c; ++d) {
+                  uint32_t w[16];
+                  tmem_ld16(tP + d * 16, w);
+#pragma unroll
+                  for (int k = 0; k < 16; ++k) {
+                    const float2 e = unpack2<kBF16>(w[k]);
+                    w[k] = pack2<kBF16>(e.x * f, e.y * f);
+                  }
+                  tmem_st16(tP + d * 16, w);
+                }
+              }
+              const float m_use = m_run == -INFINITY ? 0.f : m_run;
+              const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
+              const float2 nm2 = make_float2(-m_use, -m_use);
 #pragma unroll
               for (int k = 0; k < 16; ++k) {
-                const int gi = c * 16 + k;  // column pair of the row
-                const float2 z = __ffma2_rn(make_float2(xs[2 * gi], xs[2 * gi + 1]), sc2, nm2);
+                const float2 z = __ffma2_rn(
+                    make_float2(__uint_as_float(uc[2 * k]), __uint_as_float(uc[2 * k + 1])), sc2, nm2);
                 const float2 e = make_float2(ex2(z.x), ex2(z.y));
                 acc[k & 3] = __fadd2_rn(acc[k & 3], e);
                 pk[k] = pack2<kBF16>(e.x, e.y);
@@ -323,9 +352,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           }
           if (!ok) break;
           const float2 a01 = __fadd2_rn(__fadd2_rn(acc[0], acc[1]), __fadd2_rn(acc[2], acc[3]));
-          l_run = l_run * alpha + (a01.x + a01.y);
-          if (__any_sync(0xffffffffu, rescale)) {  // rows that do not need it multiply by 1
-            uint32_t u[2][32];
+          l_run += a01.x + a01.y;
+          if (rescale && t > it.t0) {  // rows that do not need it multiply by 1
             tmem_ld32_async(tO, u[0]);
             tmem_ld32_async(tO + 32, u[1]);
             tmem_ld_wait();
