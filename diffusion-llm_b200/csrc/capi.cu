@@ -1198,15 +1198,17 @@ int check_pages(int64_t B, int64_t Hkv, int64_t num_pages, int64_t page_size, in
 int64_t gcd64(int64_t a, int64_t b) { return b == 0 ? a : gcd64(b, a % b); }
 
 constexpr int kPagedCtas = 2;  // CTAs an SM of paged_attn_kernel (paged_attn_tc_kernel: 1)
+// workers an SM at most
+constexpr int kPagedWorkers = bd3::kPtWorkers > kPagedCtas ? bd3::kPtWorkers : kPagedCtas;
 
 // Rows per sequence and KV head up to which paged_attn_kernel takes a call.
 constexpr int64_t kPagedMaxRows = 32;
 
 // Counts (zero between calls), then the partials of the widest kernel's row tile.
-size_t paged_counter_bytes(int sms) { return static_cast<size_t>(2 * kPagedCtas * sms) * 4 + 256; }
+size_t paged_counter_bytes(int sms) { return (static_cast<size_t>(2 * kPagedWorkers * sms) * 4 + 255) / 256 * 256; }
 size_t paged_workspace_bytes(int sms) {
   const size_t rows = static_cast<size_t>(2 * kPagedCtas * sms) * 32 * 66 * 4;
-  const size_t tc = static_cast<size_t>(2 * 2 * sms) * bd3::kPtSlot * 4;
+  const size_t tc = static_cast<size_t>(2 * bd3::kPtWorkers * sms) * bd3::kPtSlot * 4;
   return paged_counter_bytes(sms) + (rows > tc ? rows : tc);
 }
 }  // namespace

@@ -26,9 +26,10 @@
 namespace bd3 {
 
 constexpr int kPtBM = 128, kPtBN = 128;
+constexpr int kPtWorkers = 2;
 constexpr int kPtStages = 3;
 constexpr int kPtThreads = 384;
-constexpr int kPtItemCost = 2;     // an item's fixed cost in key tiles
+constexpr int kPtItemCost = 3;     // an item's fixed cost in key tiles
 constexpr int kPtSlot = 128 * 66;  // floats of a partial: m[128], l[128], O[16][128] float4
 
 struct PtSmem {
@@ -143,7 +144,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           const int t = live ? r / p.G : 0;
           const uint16_t* src = reinterpret_cast<const uint16_t*>(p.q) + (it.s.q0 + t) * p.q_st +
                                 (it.h * p.G + (live ? r - t * p.G : 0)) * p.q_sh + c * 8;
-          cp_async16(wbase + PtSmem::kQ + sw128_offset(row, c), src, live);
+          cp_async16(wbase + PtSmem::kQ + sw128_offset(row ^ (64 * x), c), src, live);
         }
         return true;
       };
@@ -243,7 +244,9 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     __syncwarp();
   } else {
     // ---------------- softmax ----------------
-    const int row = threadIdx.x & 127;
+    // TMEM lane t holds row t of worker 0's tiles and row t ^ 64 of worker 1's, so that the rows of
+    // two short items (64 or fewer) keep all four of the SM's sub-partitions busy
+    const int lane128 = threadIdx.x & 127, row = lane128 ^ (64 * x);
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + lane_base + x * 128;
     const uint32_t tP = tmem + lane_base + 256 + x * 64;
@@ -374,8 +377,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           const int st = J % kPtStages;
           ok = mbar_wait_warp(&v_full[st], (J / kPtStages) & 1);
           if (!ok) break;
-          if (row >= it.hi - s) {
-            uint8_t* v = wsm + PtSmem::kV + st * kTile16 + row * 128;
+          if (lane128 >= it.hi - s) {
+            uint8_t* v = wsm + PtSmem::kV + st * kTile16 + lane128 * 128;
 #pragma unroll
             for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(v + 16 * c) = make_uint4(0, 0, 0, 0);
           }
@@ -415,7 +418,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         }
         // the share that finishes last merges the item's partials, in list order
         asm volatile("bar.sync %0, 128;" ::"r"(1 + x) : "memory");
-        if (row == 0) {
+        if (lane128 == 0) {
           __threadfence();
           const int before = atomicAdd(&p.counters[it.slot0], 1);
           *last_flag = before == it.parts - 1;

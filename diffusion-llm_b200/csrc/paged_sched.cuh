@@ -151,16 +151,16 @@ __device__ __forceinline__ int paged_part_slot(const PagedItem& it, int j) {
 }
 
 struct PagedScan {
-  long long warp_sum[16];
-  long long base[2];
-  int b[2], i[2];
+  long long warp_sum[18];
+  long long base[3];
+  int b[3], i[3];
 };
 
 // The chunk of worker kWorkers * blockIdx.x + x, found by all kThreads threads of the CTA for all
 // its workers at once; ends with a barrier. The chunk is empty for a worker past the list.
 template <int kThreads, int kWorkers, int kBM, int kBN, int kItemCost>
 __device__ __forceinline__ PagedCursor paged_chunk(const PagedParams& p, PagedScan* sc, int x) {
-  static_assert(kThreads <= 512 && kWorkers <= 2, "PagedScan");
+  static_assert(kThreads <= 576 && kWorkers <= 3, "PagedScan");
   const int pairs = p.B * p.row_tiles;
   const int per = cdiv(pairs, kThreads);
   const int e0 = imin(static_cast<int>(threadIdx.x) * per, pairs), e1 = imin(e0 + per, pairs);
