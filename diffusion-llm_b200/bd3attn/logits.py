@@ -9,10 +9,14 @@ as bits. All arguments stay on the device, so the call can be part of a captured
 
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
-from bd3attn._lib import LIB, check, i64_array
-from bd3attn.ops import _check_cuda, _code, _on_device
+from bd3attn._lib import LIB, check
+from bd3attn.ops import _check_cuda, _code, _raw_stream
+
+_I64x2, _I64x4 = ctypes.c_int64 * 2, ctypes.c_int64 * 4
 
 
 def _per_sequence(name, t, B):
@@ -51,15 +55,20 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None,
     int32 words of 32 tokens (pack_mask), (batch, words) or (batch, seq, words).
     """
     _check_cuda(logits)
+    dev = logits.device
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return process_logits(logits, history, history_len, repetition, presence, frequency,
+                                  bias, allowed, out)
     if logits.dim() != 3:
         raise AssertionError("logits must be (batch, seq, vocab)")
     B, S, V = logits.shape
     if logits.stride(2) != 1 and V > 1:
         logits = logits.contiguous()
     if out is None:
-        out = torch.empty((B, S, V), dtype=logits.dtype, device=logits.device)
+        out = torch.empty_like(logits, memory_format=torch.contiguous_format)
     elif out.shape != logits.shape or out.dtype != logits.dtype or (out.stride(2) != 1 and V > 1) \
-            or out.device != logits.device:
+            or out.device != dev:
         raise AssertionError("out must be like logits, its vocabulary contiguous")
     h_ptr = hl_ptr = None
     h_i32 = h_stride = h_cap = 0
@@ -91,15 +100,15 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None,
                 or (allowed.stride(-1) != 1 and words > 1):
             raise AssertionError("allowed must be (batch, words) or (batch, seq, words) int32")
         a_ptr = allowed.data_ptr()
-        a_strides = i64_array((allowed.stride(0), allowed.stride(1) if allowed.dim() == 3 else 0))
+        a_strides = _I64x2(allowed.stride(0), allowed.stride(1) if allowed.dim() == 3 else 0)
     if B == 0 or S == 0:
         return out
-    dev = logits.device
-    check("bd3_process_logits", _on_device(
-        dev, LIB.bd3_process_logits, logits.data_ptr(), out.data_ptr(),
-        i64_array((logits.stride(0), logits.stride(1), out.stride(0), out.stride(1))), B, S, V,
+    rc = LIB.bd3_process_logits(
+        logits.data_ptr(), out.data_ptr(),
+        _I64x4(logits.stride(0), logits.stride(1), out.stride(0), out.stride(1)), B, S, V,
         h_ptr, h_i32, h_stride, h_cap, hl_ptr, _per_sequence("repetition", repetition, B),
         _per_sequence("presence", presence, B), _per_sequence("frequency", frequency, B), b_ptr,
-        b_stride, a_ptr, a_strides, _code(logits.dtype),
-        torch.cuda.current_stream(dev).cuda_stream))
+        b_stride, a_ptr, a_strides, _code(logits.dtype), _raw_stream(dev))
+    if rc:
+        check("bd3_process_logits", rc)
     return out

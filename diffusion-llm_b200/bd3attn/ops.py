@@ -377,32 +377,35 @@ def _(qkv, n_heads, cos_table, sin_table, k_cache, v_cache, row0, positions=None
 
 # ---------------------------------------------------------------------------------------
 # Paged KV cache
-def _on_device(device, fn, *args):
-    """fn(*args) with `device` current (the context manager only where it changes something)."""
-    if torch.cuda.current_device() == device.index:
-        return fn(*args)
-    with torch.cuda.device(device):
-        return fn(*args)
+# These calls are short enough for the host's part to matter: array types are made once, the
+# stream is read as a plain handle, and the device context is entered only where it changes
+# something.
+_I64x9, _I64x11 = ctypes.c_int64 * 9, ctypes.c_int64 * 11
+
+
+def _raw_stream(device: torch.device) -> int:
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _check_pages(k_pages, v_pages, page_table, kv_lens, cu_q, dtype, n_kv_heads, D):
     _check_cuda(k_pages, v_pages, page_table, kv_lens, cu_q)
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.shape[1] != n_kv_heads \
-            or k_pages.shape[3] != D:
+    ks = k_pages.shape
+    if len(ks) != 4 or ks != v_pages.shape or ks[1] != n_kv_heads or ks[3] != D:
         raise AssertionError("k_pages and v_pages must be (pages, kv heads, page size, head_dim)")
     if k_pages.dtype != dtype or v_pages.dtype != dtype:
         raise AssertionError("k_pages and v_pages must be in the new tokens' dtype")
-    if k_pages.stride(3) != 1 or v_pages.stride(3) != 1:
-        raise AssertionError("the pages' head_dim must be contiguous")
     if page_table.dtype != torch.int32 or kv_lens.dtype != torch.int32 \
             or cu_q.dtype != torch.int32:
         raise AssertionError("page_table, kv_lens and cu_q must be int32")
-    B = kv_lens.shape[0]
-    if page_table.dim() != 2 or page_table.shape[0] != B or page_table.stride(1) != 1 \
-            or cu_q.shape != (B + 1,) or kv_lens.dim() != 1 or not cu_q.is_contiguous() \
-            or not kv_lens.is_contiguous():
+    B = kv_lens.shape[0] if kv_lens.dim() == 1 else -1
+    if page_table.dim() != 2 or page_table.shape[0] != B or cu_q.shape != (B + 1,) \
+            or not cu_q.is_contiguous() or not kv_lens.is_contiguous() \
+            or (page_table.stride(1) != 1 and page_table.shape[1] > 1):
         raise AssertionError("page_table must be (B, pages), kv_lens (B,) and cu_q (B + 1,)")
-    return B
+    kst, vst = k_pages.stride(), v_pages.stride()
+    if kst[3] != 1 or vst[3] != 1:
+        raise AssertionError("the pages' head_dim must be contiguous")
+    return B, kst, vst
 
 
 def paged_workspace(device=None) -> torch.Tensor:
@@ -431,33 +434,41 @@ def paged_attn_raw(q, k_pages, v_pages, page_table, kv_lens, cu_q, max_q_len: in
     zeroed one). Returns O (tokens, q heads, 64), with the LSE (tokens, q heads) if asked.
     """
     _check_cuda(q)
+    dev = q.device
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return paged_attn_raw(q, k_pages, v_pages, page_table, kv_lens, cu_q, max_q_len,
+                                  block_size, scale, out_dtype, return_lse, workspace)
     if q.dim() != 3:
         raise AssertionError("q must be (tokens, q heads, head_dim)")
     T, Hq, D = q.shape
-    Hkv = k_pages.shape[1]
-    B = _check_pages(k_pages, v_pages, page_table, kv_lens, cu_q, q.dtype, Hkv, D)
-    if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
+    n_pages, Hkv, page_size = k_pages.shape[:3] if k_pages.dim() == 4 else (0, 0, 0)
+    B, ks, vs = _check_pages(k_pages, v_pages, page_table, kv_lens, cu_q, q.dtype, Hkv, D)
+    qs = q.stride()
+    if qs[2] != 1 or qs[0] % 8 or qs[1] % 8 or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
+        qs = q.stride()
     code = _code(q.dtype)
-    out_dtype = q.dtype if out_dtype is None else out_dtype
-    dev = q.device
-    o = torch.empty((T, Hq, D), dtype=out_dtype, device=dev)
+    if out_dtype is None or out_dtype == q.dtype:
+        o, out_code = torch.empty_like(q, memory_format=torch.contiguous_format), code
+    else:
+        o, out_code = torch.empty((T, Hq, D), dtype=out_dtype, device=dev), _code(out_dtype)
     lse = torch.empty((T, Hq), dtype=torch.float32, device=dev) if return_lse else None
     if workspace is None:
         workspace = paged_workspace(dev)
     elif workspace.device != dev:
         raise AssertionError("the workspace must be on q's device")
-    ks, vs = k_pages.stride(), v_pages.stride()
-    strides = i64_array((q.stride(0), q.stride(1), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
-                         Hq * D, D, page_table.stride(0)))
-    check("bd3_paged_attn", _on_device(
-        dev, LIB.bd3_paged_attn, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-        o.data_ptr(), lse.data_ptr() if return_lse else None, page_table.data_ptr(),
-        kv_lens.data_ptr(), cu_q.data_ptr(), B, T, int(max_q_len), Hq, Hkv, D, k_pages.shape[0],
-        k_pages.shape[2], page_table.shape[1], strides, int(block_size),
-        D ** -0.5 if scale is None else float(scale), code, _code(out_dtype),
-        workspace.data_ptr(), workspace.numel() * workspace.element_size(),
-        torch.cuda.current_stream(dev).cuda_stream))
+    rc = LIB.bd3_paged_attn(
+        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), o.data_ptr(),
+        lse.data_ptr() if return_lse else None, page_table.data_ptr(), kv_lens.data_ptr(),
+        cu_q.data_ptr(), B, T, int(max_q_len), Hq, Hkv, D, n_pages, page_size,
+        page_table.shape[1],
+        _I64x11(qs[0], qs[1], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], Hq * D, D,
+                page_table.stride(0)),
+        int(block_size), D ** -0.5 if scale is None else float(scale), code, out_code,
+        workspace.data_ptr(), workspace.nbytes, _raw_stream(dev))
+    if rc:
+        check("bd3_paged_attn", rc)
     return (o, lse) if return_lse else o
 
 
@@ -471,32 +482,38 @@ def qkv_rope_paged_raw(qkv, n_heads: int, n_kv_heads: int, cos_table, sin_table,
     being written). The rotation is fp32, rounded once.
     """
     _check_cuda(qkv, cos_table, sin_table)
-    if qkv.dim() != 2 or qkv.shape[1] % (n_heads + 2 * n_kv_heads):
+    dev = qkv.device
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return qkv_rope_paged_raw(qkv, n_heads, n_kv_heads, cos_table, sin_table, k_pages,
+                                      v_pages, page_table, kv_lens, cu_q, q_out)
+    heads = n_heads + 2 * n_kv_heads
+    if qkv.dim() != 2 or qkv.shape[1] % heads:
         raise AssertionError("qkv must be (tokens, (n_heads + 2 * n_kv_heads) * head_dim)")
-    T = qkv.shape[0]
-    D = qkv.shape[1] // (n_heads + 2 * n_kv_heads)
-    B = _check_pages(k_pages, v_pages, page_table, kv_lens, cu_q, qkv.dtype, n_kv_heads, D)
+    T, F = qkv.shape
+    D = F // heads
+    B, ks, vs = _check_pages(k_pages, v_pages, page_table, kv_lens, cu_q, qkv.dtype, n_kv_heads, D)
     if cos_table.dtype != torch.float32 or sin_table.dtype != torch.float32 \
             or cos_table.shape != sin_table.shape or cos_table.shape[1:] != (D // 2,) \
             or not cos_table.is_contiguous() or not sin_table.is_contiguous():
         raise AssertionError("cos_table and sin_table must be contiguous (max_pos, head_dim / 2) fp32")
     if qkv.stride(1) != 1 or qkv.stride(0) * qkv.element_size() % 16 or qkv.data_ptr() % 16:
         qkv = qkv.clone(memory_format=torch.contiguous_format)
-    dev = qkv.device
     if q_out is None:
-        q_out = torch.empty((T, n_heads, D), dtype=qkv.dtype, device=dev)
+        q_out = qkv.new_empty((T, n_heads, D))
     elif q_out.shape != (T, n_heads, D) or q_out.dtype != qkv.dtype or q_out.stride(2) != 1 \
             or q_out.device != dev:
         raise AssertionError("q_out must be (tokens, n_heads, head_dim) in qkv's dtype")
-    ks, vs = k_pages.stride(), v_pages.stride()
-    strides = i64_array((q_out.stride(0), q_out.stride(1), ks[0], ks[1], ks[2], vs[0], vs[1],
-                         vs[2], page_table.stride(0)))
-    check("bd3_qkv_rope_paged", _on_device(
-        dev, LIB.bd3_qkv_rope_paged, qkv.data_ptr(), qkv.stride(0), T, B, n_heads, n_kv_heads, D,
-        cos_table.data_ptr(), sin_table.data_ptr(), cos_table.shape[0], q_out.data_ptr(),
-        k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), kv_lens.data_ptr(),
-        cu_q.data_ptr(), k_pages.shape[0], k_pages.shape[2], page_table.shape[1], strides,
-        _code(qkv.dtype), torch.cuda.current_stream(dev).cuda_stream))
+    rc = LIB.bd3_qkv_rope_paged(
+        qkv.data_ptr(), qkv.stride(0), T, B, n_heads, n_kv_heads, D, cos_table.data_ptr(),
+        sin_table.data_ptr(), cos_table.shape[0], q_out.data_ptr(), k_pages.data_ptr(),
+        v_pages.data_ptr(), page_table.data_ptr(), kv_lens.data_ptr(), cu_q.data_ptr(),
+        k_pages.shape[0], k_pages.shape[2], page_table.shape[1],
+        _I64x9(q_out.stride(0), q_out.stride(1), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
+               page_table.stride(0)),
+        _code(qkv.dtype), _raw_stream(dev))
+    if rc:
+        check("bd3_qkv_rope_paged", rc)
     return q_out
 
 
