@@ -1383,6 +1383,36 @@ int bd3_qkv_rope_paged(const void* qkv, int64_t qkv_stride, int64_t T, int64_t B
                     static_cast<cudaStream_t>(stream), "qkv_rope_paged_kernel launch", p);
 }
 
+extern "C++" {  // the launchers are templates
+namespace {
+template <int kDtype, int kU, int kR>
+int launch_logits_u(bd3::LogitParams& p, int64_t B, int sms, void* stream) {
+  using T = bd3::LogitTile<kDtype, kU>;
+  const int64_t span = (p.V + 2 * (T::kE - 1)) / T::kE * T::kE;  // chunks that start early
+  const int64_t slices = (span + T::kSlice - 1) / T::kSlice;
+  // rows per CTA: all of a sequence's (one table of its history serves them), fewer where that
+  // leaves SMs idle
+  int64_t rows = p.S;
+  while (rows > 1 && slices * B * ((p.S + rows - 1) / rows) < 4 * sms) rows = (rows + 1) / 2;
+  const int64_t z = (p.S + rows - 1) / rows;
+  if (z > 65535) return fail(BD3_ERR_UNSUPPORTED, "too many rows");
+  p.rows = static_cast<int>(rows);
+  return launch_pdl(bd3::logits_kernel<kDtype, kU, kR>,
+                    dim3(static_cast<unsigned>(slices), static_cast<unsigned>(B), static_cast<unsigned>(z)),
+                    dim3(bd3::kLogitThreads), 0, static_cast<cudaStream_t>(stream),
+                    "logits_kernel launch", p);
+}
+template <int kDtype>
+int launch_logits(bd3::LogitParams& p, int64_t B, int sms, void* stream) {
+  if (p.S > 1) return launch_logits_u<kDtype, 1, 4>(p, B, sms, stream);
+  constexpr int kSlice1 = bd3::LogitTile<kDtype, 1>::kSlice;
+  const int64_t ctas = (p.V + kSlice1 - 1) / kSlice1 * B;  // at one chunk a thread
+  return ctas >= 8LL * sms ? launch_logits_u<kDtype, 2, 1>(p, B, sms, stream)
+                           : launch_logits_u<kDtype, 1, 1>(p, B, sms, stream);
+}
+}  // namespace
+}  // extern "C++"
+
 int bd3_process_logits(const void* logits, void* out, const int64_t* strides, int64_t B,
                        int64_t S, int64_t V, const void* history, int history_is_i32,
                        int64_t history_stride, int64_t history_cap, const int32_t* history_len,
@@ -1426,24 +1456,13 @@ int bd3_process_logits(const void* logits, void* out, const int64_t* strides, in
   p.allowed = allowed;
   p.a_sb = allowed != nullptr ? allowed_strides[0] : 0;
   p.a_ss = allowed != nullptr ? allowed_strides[1] : 0;
-  p.B = static_cast<int>(B);
   p.S = static_cast<int>(S);
   p.V = static_cast<int>(V);
-  const int64_t span = (V + 14) / 8 * 8;  // chunks of 8 that start up to 7 logits early
-  p.slice = 4096;
-  while (p.slice > 1024 && (span + p.slice - 1) / p.slice * B < 2 * sms) p.slice /= 2;
-  p.n_slices = static_cast<int>((span + p.slice - 1) / p.slice);
-  p.rows = static_cast<int>(S);
-  while (p.rows > 1 && p.n_slices * B * ((S + p.rows - 1) / p.rows) < 2 * sms) p.rows = (p.rows + 1) / 2;
-  auto kern = dtype == BD3_BF16  ? bd3::logits_kernel<0>
-              : dtype == BD3_F16 ? bd3::logits_kernel<1>
-                                 : bd3::logits_kernel<2>;
-  const int64_t z = (S + p.rows - 1) / p.rows;
-  if (z > 65535) return fail(BD3_ERR_UNSUPPORTED, "too many rows");
-  const uint32_t smem = static_cast<uint32_t>(bd3::logit_smem_words(p.slice)) * 4;
-  return launch_pdl(kern, dim3(static_cast<unsigned>(p.n_slices), static_cast<unsigned>(B), static_cast<unsigned>(z)),
-                    dim3(bd3::kLogitThreads), smem, static_cast<cudaStream_t>(stream),
-                    "logits_kernel launch", p);
+  switch (dtype) {
+    case BD3_BF16: return launch_logits<0>(p, B, sms, stream);
+    case BD3_F16: return launch_logits<1>(p, B, sms, stream);
+    default: return launch_logits<2>(p, B, sms, stream);
+  }
 }
 
 int bd3_profile_enable(int on) {

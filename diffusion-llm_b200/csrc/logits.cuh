@@ -7,13 +7,19 @@
 // in fp32, each product, quotient and sum rounded to fp32, the result rounded once to the
 // logits' type. The S rows of a sequence (a block of a denoising step) share its history.
 //
-// DRAM-bound: every logit is read and written once. A CTA takes a slice of the vocabulary for some
-// rows of one sequence: it counts the history's tokens of its slice in shared memory (integer
-// atomics: the order does not matter) with a bitmap of the tokens seen, stages the bias of the
-// slice, and streams the rows through. A thread takes 8 consecutive logits with 16-byte
-// accesses; rows of an odd vocabulary start at any alignment, so its chunks begin `a` logits
-// before the multiples of 8, a being the row's misalignment. Eight tokens that the mask
-// forbids are not read.
+// DRAM-bound: every logit is read and written once, 16 bytes an access; a chunk of eight (four in
+// fp32) tokens that the mask forbids is not read. The streaming has 25 to 30 cycles of an SM
+// sub-partition for 32 chunks, so what is the same for several rows is worked out once. A CTA
+// takes a slice of the vocabulary, kU chunks a thread, for some rows of one sequence. Rows of an
+// odd vocabulary start at any alignment, so a row's chunks begin `a` logits before the
+// multiples of the chunk, a being its misalignment, which repeats every `period` rows: the CTA
+// takes the rows of one alignment together, with their mask, bias and hits of the history in
+// registers, kR rows' loads at a time. (The two ends of a row go one logit at a time.)
+// The history's tokens of the slice are counted in shared memory behind the first loads (integer
+// atomics: their order does not matter) and listed. The streaming leaves the listed tokens as
+// they were; then the CTA's threads take (token, row) pairs from the list, all lanes at work.
+// (Penalising them while streaming had one or two lanes of a warp divide at a time and took two
+// thirds of all instructions.)
 #pragma once
 
 #include "kv_rope.cuh"
@@ -21,7 +27,6 @@
 namespace bd3 {
 
 constexpr int kLogitThreads = 256;
-constexpr int kLogitSlice = 8192;  // tokens per CTA at most
 
 struct LogitParams {
   const void* logits;          // (B, S, V), vocabulary contiguous
@@ -38,131 +43,247 @@ struct LogitParams {
   long long bias_sb;
   const uint32_t* allowed;     // bit v % 32 of word v / 32; strides 0 where shared; or null
   long long a_sb, a_ss;
-  int B, S, V;
-  int slice;                   // tokens per CTA, a multiple of 8
-  int n_slices, rows;          // rows per CTA
+  int S, V;
+  int rows;                    // rows per CTA
 };
 
-// Where value x of the slice's bias sits: 8 values and a gap, so that lanes reading value c of
-// consecutive groups of 8 hit different banks.
-__device__ __forceinline__ int bias_at(int x) { return x + (x >> 3); }
+template <int kDtype, int kU>
+struct LogitTile {
+  static constexpr int kBytes = kDtype == 2 ? 4 : 2;
+  static constexpr int kE = 16 / kBytes;                     // logits of a chunk
+  static constexpr int kSlice = kLogitThreads * kU * kE;     // tokens of a CTA
+  static constexpr int kSpan = kSlice + kE;                  // its chunks start up to kE - 1 early
+  // shared words: counts, then the bitmap (one word more for the funnel shift)
+  static constexpr int kSeen = kSpan, kWords = kSeen + kSpan / 32 + 2;
+  static_assert(kSpan <= 65536, "the list holds 16-bit positions");
+};
 
-__host__ __device__ constexpr int logit_smem_words(int slice) {
-  // counts, bitmap (one word more for the funnel shift), bias: of slice + 8 tokens each
-  return (slice + 8) + ((slice + 8) / 32 + 2) + ((slice + 8) / 8 * 9 + 1);
-}
-
-template <int kDtype>
-__device__ __forceinline__ void store_logit(void* row, long long v, float x) {
-  if constexpr (kDtype == 2) reinterpret_cast<float*>(row)[v] = x;
-  else reinterpret_cast<uint16_t*>(row)[v] = static_cast<uint16_t>(pack2<kDtype == 0>(x, x));
-}
 template <int kDtype>
 __device__ __forceinline__ float load_logit(const void* row, long long v) {
   if constexpr (kDtype == 0) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(row)[v]);
   else if constexpr (kDtype == 1) return __half2float(reinterpret_cast<const __half*>(row)[v]);
   else return reinterpret_cast<const float*>(row)[v];
 }
-
+// A value as the bits of its type.
 template <int kDtype>
-__global__ void __launch_bounds__(kLogitThreads) logits_kernel(const LogitParams p) {
-  extern __shared__ uint32_t lsm[];
-  constexpr int kBytes = kDtype == 2 ? 4 : 2;
-  constexpr int kVec = 16 / kBytes;  // logits of a 16-byte access
+__device__ __forceinline__ uint32_t logit_bits(float x) {
+  if constexpr (kDtype == 2) return __float_as_uint(x);
+  else return pack2<kDtype == 0>(x, 0.f);  // the second value is in the high half: 0
+}
+
+__device__ __forceinline__ float penalise(float x, float n, float rep, float freq, float pres) {
+  const float y = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
+  return __fsub_rn(y, __fadd_rn(__fmul_rn(freq, n), pres));
+}
+
+template <int kDtype, int kU, int kR>
+__global__ void __launch_bounds__(kLogitThreads, 4) logits_kernel(const LogitParams p) {
+  using T = LogitTile<kDtype, kU>;
+  constexpr int kE = T::kE;
+  constexpr uint32_t kAll = (1u << kE) - 1u;
+  __shared__ uint32_t lsm[T::kWords];
+  __shared__ uint16_t list[T::kSpan];  // the slice's tokens that the history holds
+  __shared__ int n_list;
+  uint32_t* const count = lsm;
+  uint32_t* const seen = lsm + T::kSeen;
   griddep_wait();
   griddep_launch_dependents();
-  const int b = blockIdx.y, sl = blockIdx.x;
-  // tokens [base, base + slice + 8): the slice's chunks start up to 7 tokens early
-  const int k0 = sl * (p.slice / 8), base = 8 * k0 - 8, span = p.slice + 8;
-  uint32_t* count = lsm;
-  uint32_t* seen = count + span;
-  float* s_bias = reinterpret_cast<float*>(seen + span / 32 + 2);
+  const int b = blockIdx.y, k0 = blockIdx.x * (T::kSlice / kE);
+  const int base = (k0 - 1) * kE;  // token of the span's first count
+  const int s0 = blockIdx.z * p.rows, s1 = min(s0 + p.rows, p.S);
+  const uint8_t* const in0 = reinterpret_cast<const uint8_t*>(p.logits) + b * p.l_sb * T::kBytes;
+  uint8_t* const out0 = reinterpret_cast<uint8_t*>(p.out) + b * p.o_sb * T::kBytes;
+  const uint32_t* const mask0 = p.allowed ? p.allowed + b * p.a_sb : nullptr;
+  const bool row_mask = mask0 != nullptr && p.a_ss != 0;
+  const float* const bias = p.bias ? p.bias + b * p.bias_sb : nullptr;
   const int n_hist = p.history == nullptr ? 0 : max(0, min(p.hist_len[b], p.hist_cap));
-  if (n_hist > 0) {
-    for (int i = threadIdx.x; i < span + span / 32 + 2; i += kLogitThreads) lsm[i] = 0;
-  }
-  if (p.bias != nullptr) {
-    const float* src = p.bias + b * p.bias_sb;
-    for (int i = threadIdx.x; i < span; i += kLogitThreads) {
-      const int v = base + i;
-      s_bias[bias_at(i)] = v >= 0 && v < p.V ? src[v] : 0.f;
-    }
-  }
-  if (n_hist > 0) {
-    __syncthreads();
-    const long long h0 = b * p.h_sb;
-    for (int i = threadIdx.x; i < n_hist; i += kLogitThreads) {
-      const long long v = p.hist32 ? reinterpret_cast<const int*>(p.history)[h0 + i]
-                                   : reinterpret_cast<const long long*>(p.history)[h0 + i];
-      const long long x = v - base;
-      if (v >= 0 && v < p.V && x >= 0 && x < span) {
-        if (atomicAdd(&count[x], 1u) == 0) atomicOr(&seen[x >> 5], 1u << (x & 31));
-      }
-    }
-  }
-  __syncthreads();
   const float rep = p.repetition ? p.repetition[b] : 1.f;
   const float pres = p.presence ? p.presence[b] : 0.f;
   const float freq = p.frequency ? p.frequency[b] : 0.f;
-  const int s0 = blockIdx.z * p.rows, s1 = min(s0 + p.rows, p.S);
-  for (int s = s0; s < s1; ++s) {
-    const uint8_t* in = reinterpret_cast<const uint8_t*>(p.logits) + (b * p.l_sb + s * p.l_ss) * kBytes;
-    uint8_t* out = reinterpret_cast<uint8_t*>(p.out) + (b * p.o_sb + s * p.o_ss) * kBytes;
-    const uint32_t* mask = p.allowed ? p.allowed + b * p.a_sb + s * p.a_ss : nullptr;
-    const int a = static_cast<int>(reinterpret_cast<uintptr_t>(in) / kBytes) & (kVec - 1);
-    const bool vec_out = ((reinterpret_cast<uintptr_t>(in) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
-    const int k_end = min(k0 + p.slice / 8, (p.V + a + 7) / 8);
-    for (int k = k0 + static_cast<int>(threadIdx.x); k < k_end; k += kLogitThreads) {
-      const int v0 = 8 * k - a;
-      const int x0 = v0 - base;
-      const bool whole = v0 >= 0 && v0 + 8 <= p.V;
-      uint32_t ok = 0xFFu, hit = 0;
-      if (mask != nullptr) {
-        if (whole) {
-          ok = __funnelshift_r(mask[v0 >> 5], mask[(v0 + 7) >> 5], v0 & 31) & 0xFFu;
-        } else {
-          ok = 0;
-          for (int e = 0; e < 8; ++e) {
-            const int v = v0 + e;
-            if (v >= 0 && v < p.V) ok |= (mask[v >> 5] >> (v & 31) & 1u) << e;
+
+  // counts of the slice's tokens in the history (whole CTA)
+  auto count_history = [&]() {
+    for (int i = threadIdx.x; i < T::kWords; i += kLogitThreads) lsm[i] = 0;
+    if (threadIdx.x == 0) n_list = 0;
+    __syncthreads();
+    const long long h0 = b * p.h_sb;
+    auto add = [&](long long v) {
+      const long long x = v - base;
+      if (v >= 0 && v < p.V && x >= 0 && x < T::kSpan && atomicAdd(&count[x], 1u) == 0) {
+        atomicOr(&seen[x >> 5], 1u << (x & 31));
+        list[atomicAdd(&n_list, 1)] = static_cast<uint16_t>(x);
+      }
+    };
+    if (p.hist32) {
+      const int* h = reinterpret_cast<const int*>(p.history) + h0;
+#pragma unroll 4
+      for (int i = threadIdx.x; i < n_hist; i += kLogitThreads) add(h[i]);
+    } else {
+      const long long* h = reinterpret_cast<const long long*>(p.history) + h0;
+#pragma unroll 4
+      for (int i = threadIdx.x; i < n_hist; i += kLogitThreads) add(h[i]);
+    }
+    __syncthreads();
+  };
+  // the mask's bits of the tokens [v0, v0 + kE)
+  auto bits_of = [&](const uint32_t* m, int v0) {
+    return __funnelshift_r(m[v0 >> 5], m[(v0 + kE - 1) >> 5], v0 & 31) & kAll;
+  };
+
+  // rows of one alignment: s0 + c, s0 + c + period, ...
+  const int step = static_cast<int>(p.l_ss & (kE - 1));
+  const int period = step == 0 ? 1 : kE / (step & -step);
+  bool counted = n_hist == 0;
+  for (int c = 0; c < period && s0 + c < s1; ++c) {
+    const int a = static_cast<int>(reinterpret_cast<uintptr_t>(in0 + (s0 + c) * p.l_ss * T::kBytes) / T::kBytes) & (kE - 1);
+    int v0[kU];
+    uint32_t ok_all[kU];
+    float bv[kU][kE];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      v0[u] = (k0 + u * kLogitThreads + static_cast<int>(threadIdx.x)) * kE - a;
+      ok_all[u] = v0[u] >= 0 && v0[u] + kE <= p.V ? kAll : 0u;  // (0: an end of the row, or past it)
+      if (ok_all[u] != 0 && mask0 != nullptr && !row_mask) ok_all[u] = bits_of(mask0, v0[u]);
+    }
+    for (int sb = s0 + c; sb < s1; sb += period * kR) {
+      uint32_t ok[kR][kU];
+      uint4 raw[kR][kU];
+#pragma unroll
+      for (int r = 0; r < kR; ++r) {
+        const int s = sb + r * period;
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+          ok[r][u] = s < s1 ? ok_all[u] : 0u;
+          if (row_mask && ok[r][u] != 0) ok[r][u] = bits_of(mask0 + s * p.a_ss, v0[u]);
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < kR; ++r) {
+        const uint8_t* in = in0 + (sb + r * period) * p.l_ss * T::kBytes;
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+          raw[r][u] = make_uint4(0, 0, 0, 0);
+          if (ok[r][u] != 0)
+            raw[r][u] = *reinterpret_cast<const uint4*>(in + static_cast<long long>(v0[u]) * T::kBytes);
+        }
+      }
+      if (sb == s0 + c) {  // once for the rows of this alignment, behind the first loads
+        if (bias != nullptr) {
+#pragma unroll
+          for (int u = 0; u < kU; ++u) {
+            const float* src = bias + v0[u];
+            if (ok_all[u] == 0) continue;
+            if (reinterpret_cast<uintptr_t>(src) % 16 == 0) {
+#pragma unroll
+              for (int e = 0; e < kE; e += 4) {
+                const float4 f = *reinterpret_cast<const float4*>(src + e);
+                bv[u][e] = f.x, bv[u][e + 1] = f.y, bv[u][e + 2] = f.z, bv[u][e + 3] = f.w;
+              }
+            } else {
+#pragma unroll
+              for (int e = 0; e < kE; ++e) bv[u][e] = src[e];
+            }
+          }
+        }
+        if (!counted) {
+          count_history();
+          counted = true;
+        }
+        if (bias != nullptr && n_hist > 0) {  // listed tokens stay as they are for now
+#pragma unroll
+          for (int u = 0; u < kU; ++u) {
+            if (ok_all[u] == 0) continue;
+            const int x0 = v0[u] - base;
+            const uint32_t hit = __funnelshift_r(seen[x0 >> 5], seen[(x0 >> 5) + 1], x0 & 31);
+#pragma unroll
+            for (int e = 0; e < kE; ++e)
+              if (hit >> e & 1u) bv[u][e] = 0.f;
           }
         }
       }
-      if (n_hist > 0) hit = __funnelshift_r(seen[x0 >> 5], seen[(x0 >> 5) + 1], x0 & 31) & 0xFFu;
-      float x[8];
-      if (ok != 0) {
-        if (whole) {
-          load8<kDtype>(in, v0, x);
-        } else {
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            x[e] = v0 + e >= 0 && v0 + e < p.V ? load_logit<kDtype>(in, v0 + e) : 0.f;
-        }
-        if (hit != 0) {
+      for (int r = 0; r < kR; ++r) {
+        const int s = sb + r * period;
+        if (s >= s1) break;
+        const uint8_t* in = in0 + s * p.l_ss * T::kBytes;
+        uint8_t* out = out0 + s * p.o_ss * T::kBytes;
+        const bool vec = ((reinterpret_cast<uintptr_t>(in) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (hit >> e & 1u) {
-              const float n = static_cast<float>(count[x0 + e]);
-              const float y = x[e] > 0.f ? __fdiv_rn(x[e], rep) : __fmul_rn(x[e], rep);
-              x[e] = __fsub_rn(y, __fadd_rn(__fmul_rn(freq, n), pres));
+        for (int u = 0; u < kU; ++u) {
+          if (v0[u] >= p.V) continue;
+          if (v0[u] < 0 || v0[u] + kE > p.V) {  // an end of the row
+            const uint32_t* m = mask0 ? mask0 + s * p.a_ss : nullptr;
+#pragma unroll 1
+            for (int e = 0; e < kE; ++e) {
+              const int v = v0[u] + e;
+              if (v < 0 || v >= p.V) continue;
+              float y = -INFINITY;
+              if (m == nullptr || (m[v >> 5] >> (v & 31) & 1u)) {
+                y = load_logit<kDtype>(in, v);
+                const bool listed = n_hist > 0 && count[v - base] != 0;
+                if (bias != nullptr && !listed) y = __fadd_rn(y, bias[v]);
+              }
+              if constexpr (kDtype == 2) reinterpret_cast<float*>(out)[v] = y;
+              else reinterpret_cast<uint16_t*>(out)[v] = static_cast<uint16_t>(logit_bits<kDtype>(y));
             }
+            continue;
+          }
+          const uint4 x = raw[r][u];
+          uint32_t w[4] = {x.x, x.y, x.z, x.w};
+          if (bias != nullptr) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if constexpr (kDtype == 2) {
+                w[j] = __float_as_uint(__fadd_rn(__uint_as_float(w[j]), bv[u][j]));
+              } else {
+                const float2 f = unpack2<kDtype == 0>(w[j]);
+                w[j] = pack2<kDtype == 0>(__fadd_rn(f.x, bv[u][2 * j]), __fadd_rn(f.y, bv[u][2 * j + 1]));
+              }
+            }
+          }
+          if (mask0 != nullptr) {  // forbidden tokens
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if constexpr (kDtype == 2) {
+                if (!(ok[r][u] >> j & 1u)) w[j] = 0xFF800000u;
+              } else {
+                constexpr uint32_t kInf = kDtype == 0 ? 0xFF80FF80u : 0xFC00FC00u;
+                const uint32_t two = ok[r][u] >> (2 * j);
+                const uint32_t keep = (two & 1u) * 0xFFFFu + (two & 2u) * 0x7FFF8000u;
+                w[j] = (w[j] & keep) | (kInf & ~keep);
+              }
+            }
+          }
+          if (vec) {
+            *reinterpret_cast<uint4*>(out + static_cast<long long>(v0[u]) * T::kBytes) =
+                make_uint4(w[0], w[1], w[2], w[3]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < kE; ++e) {
+              if constexpr (kDtype == 2) reinterpret_cast<uint32_t*>(out)[v0[u] + e] = w[e];
+              else reinterpret_cast<uint16_t*>(out)[v0[u] + e] = static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1)));
+            }
+          }
         }
-        if (p.bias != nullptr) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = __fadd_rn(x[e], s_bias[bias_at(x0 + e)]);
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (!(ok >> e & 1u)) x[e] = -INFINITY;
-      if (whole && vec_out) {
-        store8<kDtype>(out, v0, x);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (v0 + e >= 0 && v0 + e < p.V) store_logit<kDtype>(out, v0 + e, x[e]);
       }
     }
+  }
+  if (n_hist == 0) return;
+  // ---- the listed tokens ----
+  __syncthreads();  // the rows are in `out`
+  const int owned = k0 * kE;  // a row's first token here is owned - a
+  const int pairs = n_list * (s1 - s0);
+  for (int i = threadIdx.x; i < pairs; i += kLogitThreads) {
+    const int r = i / n_list, s = s0 + r, x = list[i - r * n_list], v = base + x;
+    const int a = static_cast<int>(reinterpret_cast<uintptr_t>(in0 + s * p.l_ss * T::kBytes) / T::kBytes) & (kE - 1);
+    // the span's ends are the neighbour CTA's for some alignments
+    if (v < owned - a || v >= owned - a + T::kSlice) continue;
+    if (mask0 != nullptr && !(mask0[s * p.a_ss + (v >> 5)] >> (v & 31) & 1u)) continue;
+    uint8_t* out = out0 + s * p.o_ss * T::kBytes;
+    float y = penalise(load_logit<kDtype>(out, v), static_cast<float>(count[x]), rep, freq, pres);
+    if (bias != nullptr) y = __fadd_rn(y, bias[v]);
+    if constexpr (kDtype == 2) reinterpret_cast<float*>(out)[v] = y;
+    else reinterpret_cast<uint16_t*>(out)[v] = static_cast<uint16_t>(logit_bits<kDtype>(y));
   }
 }
 

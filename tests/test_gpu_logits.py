@@ -67,6 +67,9 @@ def check(d, out):
     (5, 1, 4099, 64, None, "row"), (1, 4, 33000, None, "sequence", None),
     (2, 2, 8191, None, None, "sequence"), (40, 1, 2050, 20, "vocab", None),
     (2, 1, 50257, 5000, None, None), (1, 2, 12301, None, None, None),
+    # enough sequences for two and four chunks a thread, one slice and several
+    (300, 2, 2050, 30, "vocab", "sequence"), (600, 1, 2051, 30, "sequence", "row"),
+    (40, 1, 70001, 500, "vocab", "row"), (100, 3, 25000, 100, "vocab", "sequence"),
 ], ids=lambda c: "x".join(str(v) for v in c))
 def test_matches_definition(case, dtype):
     B, S, V, cap, bias, allowed = case
