@@ -210,24 +210,7 @@ __global__ void __launch_bounds__(kLogitThreads, 4) logits_kernel(const LogitPar
         const bool vec = ((reinterpret_cast<uintptr_t>(in) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
-          if (v0[u] >= p.V) continue;
-          if (v0[u] < 0 || v0[u] + kE > p.V) {  // an end of the row
-            const uint32_t* m = mask0 ? mask0 + s * p.a_ss : nullptr;
-#pragma unroll 1
-            for (int e = 0; e < kE; ++e) {
-              const int v = v0[u] + e;
-              if (v < 0 || v >= p.V) continue;
-              float y = -INFINITY;
-              if (m == nullptr || (m[v >> 5] >> (v & 31) & 1u)) {
-                y = load_logit<kDtype>(in, v);
-                const bool listed = n_hist > 0 && count[v - base] != 0;
-                if (bias != nullptr && !listed) y = __fadd_rn(y, bias[v]);
-              }
-              if constexpr (kDtype == 2) reinterpret_cast<float*>(out)[v] = y;
-              else reinterpret_cast<uint16_t*>(out)[v] = static_cast<uint16_t>(logit_bits<kDtype>(y));
-            }
-            continue;
-          }
+          if (v0[u] < 0 || v0[u] + kE > p.V) continue;  // an end of the row, below, or past it
           const uint4 x = raw[r][u];
           uint32_t w[4] = {x.x, x.y, x.z, x.w};
           if (bias != nullptr) {
@@ -268,22 +251,59 @@ __global__ void __launch_bounds__(kLogitThreads, 4) logits_kernel(const LogitPar
       }
     }
   }
+  // ---- the ends of the rows: tokens before the first whole chunk and after the last ----
+  for (int i = threadIdx.x; i < (s1 - s0) * 2 * kE; i += kLogitThreads) {
+    const int s = s0 + i / (2 * kE), e = i % (2 * kE);
+    const uint8_t* in = in0 + s * p.l_ss * T::kBytes;
+    const int a = static_cast<int>(reinterpret_cast<uintptr_t>(in) / T::kBytes) & (kE - 1);
+    const int head = a == 0 ? 0 : min(kE - a, p.V);  // tokens [0, head) of chunk 0
+    const int last = (p.V + a) / kE;                 // chunk of the tokens after the last whole one
+    const int v = e < kE ? e : last * kE - a + e - kE;
+    const bool mine = e < kE ? k0 == 0 && v < head
+                             : last >= k0 && last < k0 + T::kSlice / kE && v >= head && v < p.V;
+    if (!mine) continue;
+    const uint32_t* m = mask0 ? mask0 + s * p.a_ss : nullptr;
+    float y = -INFINITY;
+    if (m == nullptr || (m[v >> 5] >> (v & 31) & 1u)) {
+      y = load_logit<kDtype>(in, v);
+      if (bias != nullptr && !(n_hist > 0 && count[v - base] != 0)) y = __fadd_rn(y, bias[v]);
+    }
+    uint8_t* out = out0 + s * p.o_ss * T::kBytes;
+    if constexpr (kDtype == 2) reinterpret_cast<float*>(out)[v] = y;
+    else reinterpret_cast<uint16_t*>(out)[v] = static_cast<uint16_t>(logit_bits<kDtype>(y));
+  }
   if (n_hist == 0) return;
   // ---- the listed tokens ----
   __syncthreads();  // the rows are in `out`
-  const int owned = k0 * kE;  // a row's first token here is owned - a
   const int pairs = n_list * (s1 - s0);
-  for (int i = threadIdx.x; i < pairs; i += kLogitThreads) {
-    const int r = i / n_list, s = s0 + r, x = list[i - r * n_list], v = base + x;
-    const int a = static_cast<int>(reinterpret_cast<uintptr_t>(in0 + s * p.l_ss * T::kBytes) / T::kBytes) & (kE - 1);
-    // the span's ends are the neighbour CTA's for some alignments
-    if (v < owned - a || v >= owned - a + T::kSlice) continue;
-    if (mask0 != nullptr && !(mask0[s * p.a_ss + (v >> 5)] >> (v & 31) & 1u)) continue;
-    uint8_t* out = out0 + s * p.o_ss * T::kBytes;
-    float y = penalise(load_logit<kDtype>(out, v), static_cast<float>(count[x]), rep, freq, pres);
-    if (bias != nullptr) y = __fadd_rn(y, bias[v]);
-    if constexpr (kDtype == 2) reinterpret_cast<float*>(out)[v] = y;
-    else reinterpret_cast<uint16_t*>(out)[v] = static_cast<uint16_t>(logit_bits<kDtype>(y));
+  for (int i0 = threadIdx.x; i0 < pairs; i0 += 4 * kLogitThreads) {
+    int ps[4], px[4];
+    float y[4];
+    bool live[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = i0 + j * kLogitThreads;
+      live[j] = i < pairs;
+      if (!live[j]) continue;
+      const int r = i / n_list, s = s0 + r, x = list[i - r * n_list], v = base + x;
+      const int a = static_cast<int>(reinterpret_cast<uintptr_t>(in0 + s * p.l_ss * T::kBytes) / T::kBytes) & (kE - 1);
+      // not the neighbour's (the span's ends are, for some alignments), nor forbidden
+      live[j] = v >= k0 * kE - a && v < k0 * kE - a + T::kSlice &&
+                (mask0 == nullptr || (mask0[s * p.a_ss + (v >> 5)] >> (v & 31) & 1u));
+      ps[j] = s;
+      px[j] = x;
+      if (live[j]) y[j] = load_logit<kDtype>(out0 + s * p.o_ss * T::kBytes, v);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (!live[j]) continue;
+      const int v = base + px[j];
+      y[j] = penalise(y[j], static_cast<float>(count[px[j]]), rep, freq, pres);
+      if (bias != nullptr) y[j] = __fadd_rn(y[j], bias[v]);
+      uint8_t* out = out0 + ps[j] * p.o_ss * T::kBytes;
+      if constexpr (kDtype == 2) reinterpret_cast<float*>(out)[v] = y[j];
+      else reinterpret_cast<uint16_t*>(out)[v] = static_cast<uint16_t>(logit_bits<kDtype>(y[j]));
+    }
   }
 }
 

@@ -70,6 +70,9 @@ def check(d, out):
     # enough sequences for two and four chunks a thread, one slice and several
     (300, 2, 2050, 30, "vocab", "sequence"), (600, 1, 2051, 30, "sequence", "row"),
     (40, 1, 70001, 500, "vocab", "row"), (100, 3, 25000, 100, "vocab", "sequence"),
+    # histories long enough for neighbouring CTAs to share their reading
+    (3, 5, 50259, 2500, "vocab", "row"), (70, 1, 40961, 2048, None, "sequence"),
+    (2, 1, 1500, 9000, "sequence", None),
 ], ids=lambda c: "x".join(str(v) for v in c))
 def test_matches_definition(case, dtype):
     B, S, V, cap, bias, allowed = case
