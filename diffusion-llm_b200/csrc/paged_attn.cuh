@@ -22,7 +22,7 @@ namespace bd3 {
 
 constexpr int kPgBN = 64;                      // keys per tile
 constexpr int kPgThreads = 160;                // 4 consumer warps + 1 producer warp
-constexpr int kPgItemCost = 2;                 // an item's fixed cost in tiles
+constexpr int kPgItemCost = 5;                 // an item's fixed cost in tiles
 constexpr uint32_t kPgTile = kPgBN * 128u;     // 64 keys x 128 B
 
 template <int kMB>
