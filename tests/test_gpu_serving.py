@@ -1,0 +1,123 @@
+"""Generation over the paged cache (workloads/serving.py) with a small stand-in backbone: the
+packed, chunked forward gives the logits of encoding each sequence by itself under the
+block-causal mask; grammar masks and penalties reach the drawn tokens; pages come back."""
+
+import pytest
+import torch
+
+from gpu_util import assert_device_ok
+
+pytestmark = pytest.mark.gpu
+
+V, BS = 1000, 16
+CFG = dict(d_model=128, n_heads=2, n_layers=2, d_ff=256)
+
+
+@pytest.fixture(scope="module")
+def model():
+    from workloads.backbone import Backbone
+    torch.manual_seed(0)
+    return Backbone(V, 256, BS, **CFG).cuda().bfloat16().eval()
+
+
+def full_logits(model, tokens):
+    from workloads import backbone as bb
+    bb.use_attention("sdpa")
+    n = len(tokens)
+    cos, sin = bb.rope_tables(64, n, "cuda")
+    idx = torch.arange(n, device="cuda")
+    mask = (idx[None, :] // BS) <= (idx[:, None] // BS)
+    return model.encode(tokens[None], mask, cos, sin)[0].float()
+
+
+@pytest.mark.parametrize("page_size", [16, 24, 64])
+def test_packed_chunks_match_each_sequence_alone(model, page_size):
+    from workloads.serving import PagedGeneration
+    g = torch.Generator().manual_seed(1)
+    lens = [16, 208, 64, 112]
+    seqs = [torch.randint(0, V - 1, (n,), generator=g).cuda() for n in lens]
+    gen = PagedGeneration(model, 4, 256, 80, page_size=page_size)
+    ids = [gen.cache.add() for _ in lens]
+    at, got = [0] * 4, [[] for _ in lens]
+    # uneven chunks: blocks of one sequence beside longer chunks of another, one at a time absent
+    with torch.no_grad():
+        for step in range(20):
+            take = {i: min(lens[i] - at[i], BS * (1 + (step + 3 * i) % 5)) for i in range(4)
+                    if at[i] < lens[i] and (step + i) % 4}
+            if not take:
+                continue
+            gen.cache.begin({ids[i]: n for i, n in take.items()})
+            out = gen.forward(torch.cat([seqs[i][at[i]:at[i] + n] for i, n in take.items()]))
+            gen.cache.commit()
+            for part, (i, n) in zip(out.split(list(take.values())), take.items()):
+                got[i].append(part)
+                at[i] += n
+        assert at == lens
+        assert_device_ok()
+        for i, s in enumerate(seqs):
+            ref = full_logits(model, s)
+            err = (torch.cat(got[i]).float() - ref).abs().max().item()
+            assert err <= 0.03 * max(1.0, ref.abs().max().item()), (i, err)
+
+
+def test_generation_keeps_to_the_grammar_and_returns_its_pages(model):
+    from bd3attn.logits import pack_mask
+    from workloads.serving import PagedGeneration
+    g = torch.Generator().manual_seed(2)
+    prompts = [torch.randint(0, V - 1, (n,), generator=g).cuda() for n in (32, 0, 160, 48)]
+    ok = torch.zeros(4, V, dtype=torch.bool)
+    for i in range(4):
+        ok[i, 10 * i:10 * i + 400:3] = True
+    gen = PagedGeneration(model, 4, 256, 60, page_size=16, steps=4, chunk=64, repetition=1.3,
+                          presence=0.2, frequency=0.1, bias=torch.randn(V, generator=g).cuda(), seed=3)
+    out = gen.run(prompts, [2, 3, 1, 2], pack_mask(ok).cuda())
+    assert_device_ok()
+    assert [len(o) for o in out] == [32, 48, 16, 32]
+    for i, o in enumerate(out):
+        assert ok[i][o.cpu()].all()
+    assert gen.cache.free_pages == 60
+    assert [len(o) for o in gen.run(prompts[:1], [1])] == [16]  # the cache serves again
+
+
+def test_penalties_reach_the_draw(model):
+    """With a presence penalty beyond every logit, no token of the prompt is drawn; and without
+    penalties the prompt's tokens do appear."""
+    from workloads.serving import PagedGeneration
+    prompt = torch.arange(0, V - 1).repeat_interleave(1)[:240].cuda()
+    free = [PagedGeneration(model, 1, 256, 16, steps=4, seed=s).run([prompt], [1])[0] for s in range(4)]
+    held = [PagedGeneration(model, 1, 256, 16, steps=4, seed=s, presence=1e4).run([prompt], [1])[0]
+            for s in range(4)]
+    assert_device_ok()
+    assert any((o < 240).any() for o in free) and not any((o < 240).any() for o in held)
+
+
+def test_a_captured_step_serves_growing_sequences(model):
+    """One denoising forward captured in a CUDA graph, replayed block after block as begin()
+    advances the lengths and hands out pages."""
+    from workloads.serving import PagedGeneration
+    g = torch.Generator().manual_seed(4)
+    seqs = [torch.randint(0, V - 1, (96,), generator=g).cuda() for _ in range(2)]
+    gen = PagedGeneration(model, 2, 128, 20, page_size=16)
+    ids = [gen.cache.add() for _ in seqs]
+    block = torch.zeros(2 * BS, dtype=torch.int64, device="cuda")
+    graph, logits, got = torch.cuda.CUDAGraph(), None, []
+    with torch.no_grad():
+        for b in range(6):
+            gen.cache.begin({i: BS for i in ids})
+            block.copy_(torch.cat([s[b * BS:(b + 1) * BS] for s in seqs]))
+            if b == 0:
+                side = torch.cuda.Stream()
+                side.wait_stream(torch.cuda.current_stream())
+                with torch.cuda.stream(side):
+                    gen.forward(block)
+                torch.cuda.current_stream().wait_stream(side)
+                with torch.cuda.graph(graph):
+                    logits = gen.forward(block)
+            graph.replay()
+            gen.cache.commit()
+            got.append(logits.view(2, BS, -1).clone())
+        assert_device_ok()
+        for i, s in enumerate(seqs):
+            ref = full_logits(model, s)
+            err = (torch.cat([x[i] for x in got]).float() - ref).abs().max().item()
+            assert err <= 0.03 * max(1.0, ref.abs().max().item()), (i, err)
