@@ -1285,6 +1285,9 @@ int bd3_paged_attn(const void* q, const void* k_pages, const void* v_pages, void
   p.page_size = static_cast<int>(page_size);
   p.max_pages = static_cast<int>(max_pages);
   p.bs = static_cast<int>(block_size < (1LL << 30) ? block_size : (1LL << 30));
+  p.by_G = bd3::FastDiv::of(static_cast<uint32_t>(G));
+  p.by_bs = bd3::FastDiv::of(static_cast<uint32_t>(p.bs));
+  p.by_page = bd3::FastDiv::of(static_cast<uint32_t>(page_size));
   p.out_f32 = out_dtype == BD3_F32;
   p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
   const int64_t rows = max_q * G;

@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(kPgThreads, 2)
       for (int hr = 0; hr < 2; ++hr) {
         const int r = r0 + mb * 16 + g + 8 * hr;
         const bool live = r < rows;
-        const int t = live ? r / p.G : 0;
+        const int t = live ? p.by_G.div(r) : 0;
         row_hi[mb][hr] = live ? paged_hi(p, it.s, t) : 0;
         const uint16_t* src = reinterpret_cast<const uint16_t*>(p.q) +
                               (it.s.q0 + t) * p.q_st + (it.h * p.G + (r - t * p.G)) * p.q_sh + 2 * tq;
@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(kPgThreads, 2)
           qa[mb][ks][2 + hr] = live ? *reinterpret_cast<const uint32_t*>(src + 16 * ks + 8) : 0u;
         }
       }
-    const int full_all = paged_hi(p, it.s, r0 / p.G);  // keys below this are seen by every row
+    const int full_all = paged_hi(p, it.s, p.by_G.div(r0));  // keys below this are seen by every row
 
     float acc[kMB][8][4], m_run[kMB][2], l_run[kMB][2];
 #pragma unroll
@@ -309,7 +309,7 @@ __global__ void __launch_bounds__(kPgThreads, 2)
       const float inv = L == 0.f ? 0.f : 1.f / L;  // L = 0: a row without keys
 #pragma unroll
       for (int i = 0; i < 8; ++i) o[i] *= inv;
-      const int t = r / p.G, hq = it.h * p.G + (r - t * p.G);
+      const int t = p.by_G.div(r), hq = it.h * p.G + (r - t * p.G);
       paged_store8<kBF16>(p, (it.s.q0 + t) * p.o_st + hq * p.o_sh + c8, o);
       if (p.lse != nullptr && c8 == 0)
         p.lse[static_cast<long long>(it.s.q0 + t) * (p.Hkv * p.G) + hq] =
@@ -318,13 +318,7 @@ __global__ void __launch_bounds__(kPgThreads, 2)
     if (it.parts > 1) {
       // the share that finishes last merges the item's partials, in CTA order
       asm volatile("bar.sync 1, 128;" ::: "memory");
-      if (threadIdx.x == 0) {
-        __threadfence();
-        const int before = atomicAdd(&p.counters[it.slot0], 1);
-        *last_flag = before == it.parts - 1;
-        if (before == it.parts - 1) p.counters[it.slot0] = 0;
-        __threadfence();
-      }
+      if (threadIdx.x == 0) *last_flag = paged_finish(p, it);
       asm volatile("bar.sync 1, 128;" ::: "memory");
       if (*last_flag) {
         for (int idx = threadIdx.x; idx < kRows * 8; idx += 128) {
@@ -353,7 +347,7 @@ __global__ void __launch_bounds__(kPgThreads, 2)
           const float inv = L == 0.f ? 0.f : 1.f / L;
 #pragma unroll
           for (int i = 0; i < 8; ++i) o[i] *= inv;
-          const int t = r / p.G, hq = it.h * p.G + (r - t * p.G);
+          const int t = p.by_G.div(r), hq = it.h * p.G + (r - t * p.G);
           paged_store8<kBF16>(p, (it.s.q0 + t) * p.o_st + hq * p.o_sh + c8, o);
           if (p.lse != nullptr && c8 == 0)
             p.lse[static_cast<long long>(it.s.q0 + t) * (p.Hkv * p.G) + hq] =

@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           const int row = i * 4 + (lane >> 3), c = lane & 7;
           const int r = r0 + row;
           const bool live = r < rows;
-          const int t = live ? r / p.G : 0;
+          const int t = live ? p.by_G.div(r) : 0;
           const uint16_t* src = reinterpret_cast<const uint16_t*>(p.q) + (it.s.q0 + t) * p.q_st +
                                 (it.h * p.G + (live ? r - t * p.G : 0)) * p.q_sh + c * 8;
           cp_async16(wbase + PtSmem::kQ + sw128_offset(row ^ (64 * x), c), src, live);
@@ -254,12 +254,14 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     int* const last_flag = reinterpret_cast<int*>(smem + PtSmem::kLast) + x;
     bool ok = true;
     int J = 0;  // key tiles consumed so far
-    while (paged_next<kPtBM, kPtBN, kPtItemCost>(p, cur, it)) {
+    PagedItem next;
+    for (bool more = paged_next<kPtBM, kPtBN, kPtItemCost>(p, cur, next); more;) {
+      it = next;
       const int rows = it.s.qn * p.G, r = it.i * kPtBM + row;
       const bool live = r < rows;
-      const int tok = live ? r / p.G : 0;
+      const int tok = live ? p.by_G.div(r) : 0;
       const int row_hi = live ? paged_hi(p, it.s, tok) : 0;
-      const int full_all = paged_hi(p, it.s, it.i * kPtBM / p.G);  // seen by every row
+      const int full_all = paged_hi(p, it.s, p.by_G.div(it.i * kPtBM));  // seen by every row
       const bool dead = !__any_sync(0xffffffffu, live);  // a warp without rows computes nothing
       float m_run = -INFINITY, l_run = 0.f;
       for (int t = it.t0; t < it.t1; ++t, ++J) {
@@ -394,6 +396,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         tc_fence_before();
         mbar_arrive(p_full);
       }
+      more = paged_next<kPtBM, kPtBN, kPtItemCost>(p, cur, next);  // (while the last P V runs)
       // ---- the share's end: the last O += P V has landed; O / l, or the share's partial ----
       if (ok) ok = mbar_wait_warp(o_done, (J - 1) & 1);
       if (!bar_and(1 + x, 128, ok)) break;
@@ -425,13 +428,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         }
         // the share that finishes last merges the item's partials, in list order
         asm volatile("bar.sync %0, 128;" ::"r"(1 + x) : "memory");
-        if (lane128 == 0) {
-          __threadfence();
-          const int before = atomicAdd(&p.counters[it.slot0], 1);
-          *last_flag = before == it.parts - 1;
-          if (before == it.parts - 1) p.counters[it.slot0] = 0;
-          __threadfence();
-        }
+        if (lane128 == 0) *last_flag = paged_finish(p, it);
         asm volatile("bar.sync %0, 128;" ::"r"(1 + x) : "memory");
         if (*last_flag == 0) continue;
         M = -INFINITY;

@@ -27,6 +27,22 @@
 
 namespace bd3 {
 
+// Division of 0 <= x < 2^31 by a launch constant d, as a multiplication (Granlund and Montgomery,
+// "Division by invariant integers using multiplication", PLDI 1994): with l = ceil(log2 d) and
+// m = ceil(2^(31 + l) / d) < 2^32, m d - 2^(31 + l) < 2^l, so floor(x m / 2^(31 + l)) = floor(x / d).
+struct FastDiv {
+  uint32_t m, s;  // s = l - 1; d = 1: m = 0
+  __host__ static FastDiv of(uint32_t d) {
+    if (d == 1) return FastDiv{0, 0};
+    uint32_t l = 1;
+    while ((1ull << l) < d) ++l;
+    return FastDiv{static_cast<uint32_t>(((1ull << (31 + l)) + d - 1) / d), l - 1};
+  }
+  __device__ __forceinline__ int div(int x) const {
+    return m == 0 ? x : static_cast<int>(__umulhi(static_cast<uint32_t>(x), m) >> s);
+  }
+};
+
 struct PagedParams {
   const void* q;              // (total_q, Hq, 64); token and head strides in elements
   void* o;                    // (total_q, Hq, 64) in the output dtype
@@ -42,6 +58,7 @@ struct PagedParams {
   int num_pages, page_size, max_pages;
   int box;                    // rows of one TMA piece: divides the page size and the key tile
   int bs;
+  FastDiv by_G, by_bs, by_page;  // by G, bs and page_size
   int row_tiles;              // row tiles of max_q tokens
   int out_f32;
   float scale_log2;           // softmax scale * log2(e)
@@ -69,7 +86,7 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedParams& p, int b) {
 __device__ __forceinline__ int paged_hi(const PagedParams& p, const PagedSeq& s, int t) {
   const int pos = s.kv - s.qn + t;
   if (pos < 0) return 0;
-  const long long hi = (static_cast<long long>(pos / p.bs) + 1) * p.bs;
+  const long long hi = (static_cast<long long>(p.by_bs.div(pos)) + 1) * p.bs;
   return hi < s.kv ? static_cast<int>(hi) : s.kv;
 }
 
@@ -80,7 +97,7 @@ __device__ __forceinline__ int paged_tiles(const PagedParams& p, const PagedSeq&
                                            int* hi_out) {
   const int rows = s.qn * p.G, r0 = i * kBM;
   if (r0 >= rows) return 0;
-  const int hi = paged_hi(p, s, (imin(r0 + kBM, rows) - 1) / p.G);
+  const int hi = paged_hi(p, s, p.by_G.div(imin(r0 + kBM, rows) - 1));
   *hi_out = hi;
   return hi > kBN ? (hi - 1) / kBN + 1 : 1;
 }
@@ -95,11 +112,13 @@ struct PagedItem {
   int slot;       // this share's partial
   int slot0;      // the first share's partial, and the item's count
   int w0;         // the first share's worker
+  int n;          // key tiles of the item
 };
 
 struct PagedCursor {
   int w;                      // this worker
   int b, i;
+  bool same;                  // the item holds the pair (b, i)'s s, n and hi already
   long long base;             // list position of the pair (b, i)
   long long pos, lo, end, chunk;
 };
@@ -108,17 +127,22 @@ struct PagedCursor {
 template <int kBM, int kBN, int kItemCost>
 __device__ __forceinline__ bool paged_next(const PagedParams& p, PagedCursor& c, PagedItem& it) {
   while (c.pos < c.end && c.b < p.B) {
-    it.s = paged_seq(p, c.b);
-    const int n = paged_tiles<kBM, kBN>(p, it.s, c.i, &it.hi);
-    if (n == 0) {  // past the sequence's rows
-      ++c.b;
-      c.i = 0;
-      continue;
+    if (!c.same) {
+      it.s = paged_seq(p, c.b);
+      it.n = paged_tiles<kBM, kBN>(p, it.s, c.i, &it.hi);
+      if (it.n == 0) {  // past the sequence's rows
+        ++c.b;
+        c.i = 0;
+        continue;
+      }
+      c.same = true;
     }
+    const int n = it.n;
     const int cost = n + kItemCost;
     const long long w = static_cast<long long>(cost) * p.Hkv;
     if (c.pos >= c.base + w) {
       c.base += w;
+      c.same = false;
       if (++c.i == p.row_tiles) {
         ++c.b;
         c.i = 0;
@@ -135,14 +159,30 @@ __device__ __forceinline__ bool paged_next(const PagedParams& p, PagedCursor& c,
     if (stop <= first) continue;  // only the item's fixed cost falls into this chunk
     it.t0 = static_cast<int>(from - first);
     it.t1 = static_cast<int>(stop - first);
-    const long long w0 = first / c.chunk, w1 = (first + n - 1) / c.chunk;
-    it.w0 = static_cast<int>(w0);
-    it.parts = static_cast<int>(w1 - w0) + 1;
-    it.slot0 = 2 * it.w0 + (first == w0 * c.chunk ? 0 : 1);
+    // the workers of the item's first and last tile, counted from this one (32-bit divisions:
+    // a 64-bit one costs hundreds of cycles, and every role of a worker does this per share)
+    const uint32_t chunk = c.chunk < 0x7FFFFFFF ? static_cast<uint32_t>(c.chunk) : 0x7FFFFFFFu;
+    const int before = c.lo > first ? static_cast<int>((static_cast<uint32_t>(c.lo - first) + chunk - 1u) / chunk) : 0;
+    const int after = first + n > c.end ? static_cast<int>(static_cast<uint32_t>(first + n - 1 - c.lo) / chunk) : 0;
+    it.w0 = c.w - before;
+    it.parts = before + after + 1;
+    it.slot0 = 2 * it.w0 + (first == c.lo - before * c.chunk ? 0 : 1);
     it.slot = 2 * c.w + (from == c.lo ? 0 : 1);
     return true;
   }
   return false;
+}
+// Count one more finished share of a cut item; true for the last one. For one thread, after a barrier
+// behind every thread's stores of the partial; release and acquire at device scope.
+__device__ __forceinline__ bool paged_finish(const PagedParams& p, const PagedItem& it) {
+  int before;
+  asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;"
+               : "=r"(before)
+               : "l"(&p.counters[it.slot0])
+               : "memory");
+  if (before != it.parts - 1) return false;
+  p.counters[it.slot0] = 0;
+  return true;
 }
 // Partial slot of share j of an item.
 __device__ __forceinline__ int paged_part_slot(const PagedItem& it, int j) {
@@ -222,6 +262,7 @@ __device__ __forceinline__ PagedCursor paged_chunk(const PagedParams& p, PagedSc
   c.base = sc->base[x];
   c.b = c.lo < c.end ? sc->b[x] : p.B;
   c.i = sc->i[x];
+  c.same = false;
   return c;
 }
 
@@ -237,7 +278,7 @@ __device__ __forceinline__ int paged_lookup(const PagedParams& p, const PagedIte
   const long long key = static_cast<long long>(tile + lane / pieces) * kBN + (lane % pieces) * p.box;
   *row = 0;
   if (key >= it.hi) return p.num_pages;
-  const int pg = static_cast<int>(key) / p.page_size;
+  const int pg = p.by_page.div(static_cast<int>(key));
   *row = static_cast<int>(key) - pg * p.page_size;
   const int id = p.page_table[it.b * p.pt_stride + pg];
   if (id < 0 || id >= p.num_pages) {
