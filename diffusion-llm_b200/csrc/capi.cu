@@ -3,6 +3,7 @@
 // Host side only: argument validation (mirroring the reference's assertions), TMA tensor
 // map construction, launch planning and kernel launches. No allocation happens here: the
 // caller passes every output and workspace buffer.
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -1314,6 +1315,18 @@ int bd3_paged_attn(const void* q, const void* k_pages, const void* v_pages, void
                                    : bd3::PtSmem::kAlloc;
   const unsigned threads = bm == bd3::kPtBM ? bd3::kPtThreads : bd3::kPgThreads;
   if ((rc = set_smem(kern, smem, (bm == 16 ? 0 : bm == 32 ? 2 : 4) + (bf ? 0 : 1))) != BD3_OK) return rc;
+  if (bm == bd3::kPtBM) {  // its register split needs what it was written for (see kPtRegs)
+    static std::atomic<int> regs[2];
+    int n = regs[bf].load(std::memory_order_relaxed);
+    if (n == 0) {
+      cudaFuncAttributes at;
+      const cudaError_t e = cudaFuncGetAttributes(&at, kern);
+      if (e != cudaSuccess) return cuda_fail(e, "cudaFuncGetAttributes");
+      regs[bf].store(n = at.numRegs, std::memory_order_relaxed);
+    }
+    if (n != bd3::kPtRegs)
+      return fail(BD3_ERR_CUDA, "paged attention was built with %d registers a thread, not %d", n, bd3::kPtRegs);
+  }
   return launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(threads), smem,
                     static_cast<cudaStream_t>(stream), "paged attention launch", tk, tv, p);
 }

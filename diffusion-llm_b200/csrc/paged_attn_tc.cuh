@@ -8,7 +8,13 @@
 // row max, exponentials, P store): one warpgroup alone leaves the exponential units idle for
 // most of a tile. So each SM runs two independent workers, each with its own chunk of the work
 // list, Q tile, K/V ring, TMEM columns and three roles, and nothing synchronises them: one's
-// exponentials fill the other's loads and waits. Per worker x (384 threads in all):
+// exponentials fill the other's loads and waits. (Measured on a 2048-token chunk after 8192, 12
+// heads: key columns of one tile split between the warpgroups 126 us, two workers 119 us, with
+// registers moved to the softmax 113 us. Three workers on 64-key tiles: 131 us, their rings and
+// TMEM leave each too little. The row max by 32-column chunks, ahead of or behind the
+// exponentials: 119 to 134 us. A quarter of the exponentials on the FMA pipe: 109 us there, but
+// 88 against 82 us on short prompts, whose code then no longer fits the instruction cache.)
+// Per worker x (384 threads in all):
 //   warps 4x..4x+3  softmax: thread t owns row t (TMEM lane t) and all 128 columns of a tile; at a
 //                   share's end O / l to global memory, or the share's partial
 //   warp 8 + x      producer: Q rows (token, head) by cp.async into the swizzled tile, K and V
@@ -20,7 +26,7 @@
 // voted per warp.
 #pragma once
 
-#include "attn_fwd.cuh"
+#include "attn_fwd_pair.cuh"
 #include "paged_attn.cuh"
 
 namespace bd3 {
@@ -29,7 +35,12 @@ constexpr int kPtBM = 128, kPtBN = 128;
 constexpr int kPtWorkers = 2;
 constexpr int kPtStages = 3;
 constexpr int kPtThreads = 384;
-constexpr int kPtItemCost = 3;     // an item's fixed cost in key tiles
+constexpr int kPtItemCost = 2;     // an item's fixed cost in key tiles
+// Registers a thread, of the 168 that 384 threads launch with: the softmax holds a row's 128
+// scores (at 168 it spilled), the other four warps need few. 256 x 192 + 128 x 120 = 384 x 168;
+// the host checks that the kernel has the 168 (more than the launch's own would wait for ever).
+constexpr int kPtRegs = 168, kPtRegsSoftmax = 192, kPtRegsOther = 120;
+static_assert(256 * kPtRegsSoftmax + 128 * kPtRegsOther <= kPtThreads * kPtRegs, "register split");
 constexpr int kPtSlot = 128 * 66;  // floats of a partial: m[128], l[128], O[16][128] float4
 
 struct PtSmem {
@@ -52,18 +63,6 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool l
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
                "r"(live ? 16u : 0u)
                : "memory");
-}
-// Max over 32 floats as a tree of three-input maxes.
-__device__ __forceinline__ float max32(const uint32_t (&u)[32]) {
-  float a[11], b[4];
-#pragma unroll
-  for (int i = 0; i < 10; ++i)
-    a[i] = max3(__uint_as_float(u[3 * i]), __uint_as_float(u[3 * i + 1]), __uint_as_float(u[3 * i + 2]));
-  a[10] = fmaxf(__uint_as_float(u[30]), __uint_as_float(u[31]));
-#pragma unroll
-  for (int i = 0; i < 3; ++i) b[i] = max3(a[3 * i], a[3 * i + 1], a[3 * i + 2]);
-  b[3] = fmaxf(a[9], a[10]);
-  return max3(b[0], b[1], fmaxf(b[2], b[3]));
 }
 __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
@@ -125,125 +124,129 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   const uint32_t tmem = *tmem_slot;
   PagedItem it;
 
-  if (warp >= 8 && warp < 10) {
-    // ---------------- producer ----------------
-    bool ok = true;
-    int J = 0;  // key tiles loaded so far
-    for (int n = 0; ok && paged_next<kPtBM, kPtBN, kPtItemCost>(p, cur, it); ++n) {
-      // Q: issued first for the first item, and for a later one after its first K/V tile (the Q
-      // tile is in use until the last S of the item before)
-      bool q_sent = false;
-      auto load_q = [&]() {
-        if (n > 0 && !mbar_wait_warp(q_empty, (n - 1) & 1)) return false;
-        const int rows = it.s.qn * p.G, r0 = it.i * kPtBM;
-#pragma unroll 4
-        for (int i = 0; i < 32; ++i) {
-          const int row = i * 4 + (lane >> 3), c = lane & 7;
-          const int r = r0 + row;
-          const bool live = r < rows;
-          const int t = live ? p.by_G.div(r) : 0;
-          const uint16_t* src = reinterpret_cast<const uint16_t*>(p.q) + (it.s.q0 + t) * p.q_st +
-                                (it.h * p.G + (live ? r - t * p.G : 0)) * p.q_sh + c * 8;
-          cp_async16(wbase + PtSmem::kQ + sw128_offset(row ^ (64 * x), c), src, live);
-        }
-        return true;
-      };
-      auto send_q = [&]() {  // the rows are in shared memory: hand them to the tensor cores
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(q_full);
-        q_sent = true;
-      };
-      const int J0 = J;
-      if (n == 0) ok = load_q();
-      ok = ok && paged_stream<kPtBN>(
-          p, it, J,
-          [&](int j) {
-            if (j == J0 + 1 && !q_sent) {
-              if (n > 0 && !load_q()) return false;
-              send_q();
-            }
-            const int st = j % kPtStages;
-            if (j >= kPtStages && !mbar_wait_warp(&kv_empty[st], ((j / kPtStages) - 1) & 1))
-              return false;
-            if (lane == 0) {
-              mbar_expect_tx(&k_full[st], kTile16);
-              mbar_expect_tx(&v_full[st], kTile16);
-            }
-            return true;
-          },
-          [&](int j, int piece, int page, int row) {
-            const int st = j % kPtStages;
-            const uint32_t off = st * kTile16 + piece * p.box * 128;
-            tma_load_4d(&tm_k, &k_full[st], wsm + PtSmem::kK + off, 0, row, it.h, page);
-            tma_load_4d(&tm_v, &v_full[st], wsm + PtSmem::kV + off, 0, row, it.h, page);
-          });
-      if (ok && !q_sent) {
-        if (n > 0) ok = load_q();
-        if (ok) send_q();
-      }
-    }
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    __syncwarp();
-  } else if (warp >= 10) {
-    // ---------------- UMMA issuer ----------------
-    if (elect_one()) {
-      constexpr uint32_t idesc_qk = idesc_f16(128, 128, false, false, kBF16);
-      constexpr uint32_t idesc_pv = idesc_f16(128, 64, false, true, kBF16);
-      const uint64_t qdesc = sw128_desc(wbase + PtSmem::kQ, 16, 1024);
-      bool ok = true, first = false, pending = false;
-      int J = 0, pn = 0;
-      // O += P V of tile J - 1, then release its K/V stage; the first one of item pn overwrites
-      // O, after the epilogue of the item before has read it
-      auto issue_pv = [&]() {
-        const int j = J - 1, st = j % kPtStages;
-        pending = false;
-        ok = ok && mbar_wait(&v_full[st], (j / kPtStages) & 1);
-        if (ok && first && pn > 0) ok = mbar_wait(o_free, (pn - 1) & 1);
-        ok = ok && mbar_wait(p_full, j & 1);
-        if (!ok) return;
-        tc_fence_after();
-        const uint64_t vdesc = sw128_desc(wbase + PtSmem::kV + st * kTile16, kTile16, 1024);
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
-          umma_ts(tmem + 384 + x * 64, tmem + 256 + x * 64 + kk * 8, vdesc + ((kk * 2048) >> 4),
-                  idesc_pv, (!first || kk > 0) ? 1u : 0u);
-        umma_commit(o_done);
-        umma_commit(&kv_empty[st]);
-      };
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPtRegsOther));
+    if (warp < 10) {
+      // ---------------- producer ----------------
+      bool ok = true;
+      int J = 0;  // key tiles loaded so far
       for (int n = 0; ok && paged_next<kPtBM, kPtBN, kPtItemCost>(p, cur, it); ++n) {
-        // S of a tile goes before O += P V of the one before it, so that it is ready when that
-        // tile's softmax ends; at an item's start only if its Q and K are there already
-        if (pending && !(mbar_test(q_full, n & 1) &&
-                         mbar_test(&k_full[J % kPtStages], (J / kPtStages) & 1)))
-          issue_pv();
-        ok = ok && mbar_wait(q_full, n & 1);
-        for (int t = it.t0; ok && t < it.t1; ++t) {
-          const int st = J % kPtStages;
-          ok = mbar_wait(&k_full[st], (J / kPtStages) & 1);
-          if (ok && J > 0) ok = mbar_wait(s_free, (J - 1) & 1);  // S is in registers
-          if (!ok) break;
-          tc_fence_after();
-          const uint64_t kdesc = sw128_desc(wbase + PtSmem::kK + st * kTile16, 16, 1024);
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            umma_ss(tmem + x * 128, qdesc + ((kk * 32) >> 4), kdesc + ((kk * 32) >> 4), idesc_qk,
-                    kk > 0 ? 1u : 0u);
-          umma_commit(s_full);
-          if (t == it.t1 - 1) umma_commit(q_empty);
-          if (pending) issue_pv();
-          ++J;
-          pending = true;
-          first = t == it.t0;
-          pn = n;
+        // Q: issued first for the first item, and for a later one after its first K/V tile (the Q
+        // tile is in use until the last S of the item before)
+        bool q_sent = false;
+        auto load_q = [&]() {
+          if (n > 0 && !mbar_wait_warp(q_empty, (n - 1) & 1)) return false;
+          const int rows = it.s.qn * p.G, r0 = it.i * kPtBM;
+#pragma unroll 4
+          for (int i = 0; i < 32; ++i) {
+            const int row = i * 4 + (lane >> 3), c = lane & 7;
+            const int r = r0 + row;
+            const bool live = r < rows;
+            const int t = live ? p.by_G.div(r) : 0;
+            const uint16_t* src = reinterpret_cast<const uint16_t*>(p.q) + (it.s.q0 + t) * p.q_st +
+                                  (it.h * p.G + (live ? r - t * p.G : 0)) * p.q_sh + c * 8;
+            cp_async16(wbase + PtSmem::kQ + sw128_offset(row ^ (64 * x), c), src, live);
+          }
+          return true;
+        };
+        auto send_q = [&]() {  // the rows are in shared memory: hand them to the tensor cores
+          asm volatile("cp.async.wait_all;" ::: "memory");
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(q_full);
+          q_sent = true;
+        };
+        const int J0 = J;
+        if (n == 0) ok = load_q();
+        ok = ok && paged_stream<kPtBN>(
+            p, it, J,
+            [&](int j) {
+              if (j == J0 + 1 && !q_sent) {
+                if (n > 0 && !load_q()) return false;
+                send_q();
+              }
+              const int st = j % kPtStages;
+              if (j >= kPtStages && !mbar_wait_warp(&kv_empty[st], ((j / kPtStages) - 1) & 1))
+                return false;
+              if (lane == 0) {
+                mbar_expect_tx(&k_full[st], kTile16);
+                mbar_expect_tx(&v_full[st], kTile16);
+              }
+              return true;
+            },
+            [&](int j, int piece, int page, int row) {
+              const int st = j % kPtStages;
+              const uint32_t off = st * kTile16 + piece * p.box * 128;
+              tma_load_4d(&tm_k, &k_full[st], wsm + PtSmem::kK + off, 0, row, it.h, page);
+              tma_load_4d(&tm_v, &v_full[st], wsm + PtSmem::kV + off, 0, row, it.h, page);
+            });
+        if (ok && !q_sent) {
+          if (n > 0) ok = load_q();
+          if (ok) send_q();
         }
       }
-      if (ok && pending) issue_pv();
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      __syncwarp();
+    } else {
+      // ---------------- UMMA issuer ----------------
+      if (elect_one()) {
+        constexpr uint32_t idesc_qk = idesc_f16(128, 128, false, false, kBF16);
+        constexpr uint32_t idesc_pv = idesc_f16(128, 64, false, true, kBF16);
+        const uint64_t qdesc = sw128_desc(wbase + PtSmem::kQ, 16, 1024);
+        bool ok = true, first = false, pending = false;
+        int J = 0, pn = 0;
+        // O += P V of tile J - 1, then release its K/V stage; the first one of item pn overwrites
+        // O, after the epilogue of the item before has read it
+        auto issue_pv = [&]() {
+          const int j = J - 1, st = j % kPtStages;
+          pending = false;
+          ok = ok && mbar_wait(&v_full[st], (j / kPtStages) & 1);
+          if (ok && first && pn > 0) ok = mbar_wait(o_free, (pn - 1) & 1);
+          ok = ok && mbar_wait(p_full, j & 1);
+          if (!ok) return;
+          tc_fence_after();
+          const uint64_t vdesc = sw128_desc(wbase + PtSmem::kV + st * kTile16, kTile16, 1024);
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk)
+            umma_ts(tmem + 384 + x * 64, tmem + 256 + x * 64 + kk * 8, vdesc + ((kk * 2048) >> 4),
+                    idesc_pv, (!first || kk > 0) ? 1u : 0u);
+          umma_commit(o_done);
+          umma_commit(&kv_empty[st]);
+        };
+        for (int n = 0; ok && paged_next<kPtBM, kPtBN, kPtItemCost>(p, cur, it); ++n) {
+          // S of a tile goes before O += P V of the one before it, so that it is ready when that
+          // tile's softmax ends; at an item's start only if its Q and K are there already
+          if (pending && !(mbar_test(q_full, n & 1) &&
+                           mbar_test(&k_full[J % kPtStages], (J / kPtStages) & 1)))
+            issue_pv();
+          ok = ok && mbar_wait(q_full, n & 1);
+          for (int t = it.t0; ok && t < it.t1; ++t) {
+            const int st = J % kPtStages;
+            ok = mbar_wait(&k_full[st], (J / kPtStages) & 1);
+            if (ok && J > 0) ok = mbar_wait(s_free, (J - 1) & 1);  // S is in registers
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t kdesc = sw128_desc(wbase + PtSmem::kK + st * kTile16, 16, 1024);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              umma_ss(tmem + x * 128, qdesc + ((kk * 32) >> 4), kdesc + ((kk * 32) >> 4), idesc_qk,
+                      kk > 0 ? 1u : 0u);
+            umma_commit(s_full);
+            if (t == it.t1 - 1) umma_commit(q_empty);
+            if (pending) issue_pv();
+            ++J;
+            pending = true;
+            first = t == it.t0;
+            pn = n;
+          }
+        }
+        if (ok && pending) issue_pv();
+      }
+      __syncwarp();
     }
-    __syncwarp();
   } else {
     // ---------------- softmax ----------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPtRegsSoftmax));
     // TMEM lane t holds row t of worker 0's tiles and row t ^ 64 of worker 1's, so that the rows of
     // two short items (64 or fewer) keep all four of the SM's sub-partitions busy
     const int lane128 = threadIdx.x & 127, row = lane128 ^ (64 * x);
@@ -283,89 +286,65 @@ __global__ void __launch_bounds__(kPtThreads, 1)
 #pragma unroll
           for (int c = 0; c < 4; ++c)
             if (__any_sync(0xffffffffu, hi > 32 * c)) vis |= 1u << c;
-          // 32 columns at a time, the next ones on their way from TMEM: P = 2^(x scale - m) with the
-          // m of the chunks before, unless a row's max is more than 2^8 above it (as in an
-          // item's first chunk); then m is raised and what was summed or stored under the old
-          // one is scaled down. (A loop of twice two chunks: unrolled to four it was 4% faster
-          // on long items and 12% slower on short ones, where the code of both workers' phases
-          // no longer fits the instruction cache.)
+          float xs[128];
+          uint32_t u[4][32];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld32_async(tS + c * 32, u[c]);
+          tmem_ld_wait();
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            reg_fence(u[c]);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) xs[c * 32 + k] = __uint_as_float(u[c][k]);
+          }
+          tc_fence_before();
+          mbar_arrive(s_free);  // S is in registers: the next one may be computed
+          const float mx = max3(chunk_max<0>(xs, vis, masked, 0, hi),
+                                chunk_max<1>(xs, vis, masked, 0, hi),
+                                fmaxf(chunk_max<2>(xs, vis, masked, 0, hi),
+                                      chunk_max<3>(xs, vis, masked, 0, hi))) *
+                           p.scale_log2;
+          float alpha = 1.f;
+          bool up = false;
+          const float m_new = fmaxf(m_run, mx);
+          if (m_new - m_run > kRescaleLog2) {  // false for NaN (-inf - -inf)
+            alpha = ex2(m_run - m_new);        // 0 when m_run = -inf
+            up = t > it.t0;
+            m_run = m_new;
+          }
+          const bool rescale = __any_sync(0xffffffffu, up);
+          const float m_use = m_run == -INFINITY ? 0.f : m_run;
+          const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
+          const float2 nm2 = make_float2(-m_use, -m_use);
           float2 acc[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f),
                            make_float2(0.f, 0.f)};
-          float alpha = 1.f;
-          bool rescale = false;  // the same for all lanes
-          uint32_t u[2][32];
-          tmem_ld32_async(tS, u[0]);
-#pragma unroll 1
-          for (int cc = 0; cc < 4; cc += 2) {
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-              const int c = cc + hf;
-              uint32_t(&uc)[32] = u[hf];
-              tmem_ld_wait();
-              reg_fence(uc);
-              if (c < 3) {
-                tmem_ld32_async(tS + 32 * (c + 1), u[hf ^ 1]);
-              } else {
-                tc_fence_before();
-                mbar_arrive(s_free);  // S is in registers: the next one may be computed
+          for (int c = 0; c < 4; ++c) {
+            uint32_t pk[16];
+            if (vis & (1u << c)) {
+#pragma unroll
+              for (int k = 0; k < 16; ++k) {
+                const int gi = c * 16 + k;  // column pair of the row
+                const float2 z = __ffma2_rn(make_float2(xs[2 * gi], xs[2 * gi + 1]), sc2, nm2);
+                const float2 e = make_float2(ex2(z.x), ex2(z.y));
+                acc[k & 3] = __fadd2_rn(acc[k & 3], e);
+                pk[k] = pack2<kBF16>(e.x, e.y);
               }
-              uint32_t pk[16];
-              if (vis >> c & 1u) {
-                if (masked) {
-                  const int hc = hi - 32 * c;
+            } else {
 #pragma unroll
-                  for (int k = 0; k < 32; ++k)
-                    if (k >= hc) uc[k] = 0xFF800000u;  // -inf
-                }
-                const float mx = max32(uc) * p.scale_log2;
-                const bool up = mx - m_run > kRescaleLog2;  // false for NaN (-inf - -inf)
-                if (__any_sync(0xffffffffu, up)) {
-                  const float f = up ? ex2(m_run - mx) : 1.f;  // 0 when m_run = -inf
-                  if (up) m_run = mx;
-                  alpha *= f;
-                  l_run *= f;
-                  rescale = true;
-#pragma unroll
-                  for (int i = 0; i < 4; ++i) acc[i] = __fmul2_rn(acc[i], make_float2(f, f));
-                  tmem_st_wait();
-#pragma unroll 1
-                  for (int d = 0; d < c; ++d) {
-                    uint32_t w[16];
-                    tmem_ld16(tP + d * 16, w);
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                      const float2 e = unpack2<kBF16>(w[k]);
-                      w[k] = pack2<kBF16>(e.x * f, e.y * f);
-                    }
-                    tmem_st16(tP + d * 16, w);
-                  }
-                }
-                const float m_use = m_run == -INFINITY ? 0.f : m_run;
-                const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
-                const float2 nm2 = make_float2(-m_use, -m_use);
-#pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                  const float2 z = __ffma2_rn(
-                      make_float2(__uint_as_float(uc[2 * k]), __uint_as_float(uc[2 * k + 1])), sc2, nm2);
-                  const float2 e = make_float2(ex2(z.x), ex2(z.y));
-                  acc[k & 3] = __fadd2_rn(acc[k & 3], e);
-                  pk[k] = pack2<kBF16>(e.x, e.y);
-                }
-              } else {
-#pragma unroll
-                for (int k = 0; k < 16; ++k) pk[k] = 0u;
-              }
-              if (c == 0 && t > it.t0) {
-                ok = mbar_wait_warp(o_done, (J - 1) & 1);  // the P of the tile before is used up
-                tc_fence_after();
-              }
-              tmem_st16(tP + c * 16, pk);
+              for (int k = 0; k < 16; ++k) pk[k] = 0u;
             }
+            if (c == 0 && t > it.t0) {
+              ok = mbar_wait_warp(o_done, (J - 1) & 1);  // the P of the tile before is used up
+              tc_fence_after();
+            }
+            tmem_st16(tP + c * 16, pk);
           }
+          l_run *= alpha;
           if (!ok) break;
           const float2 a01 = __fadd2_rn(__fadd2_rn(acc[0], acc[1]), __fadd2_rn(acc[2], acc[3]));
           l_run += a01.x + a01.y;
-          if (rescale && t > it.t0) {  // rows that do not need it multiply by 1
+          if (rescale) {  // rows that do not need it multiply by 1
             tmem_ld32_async(tO, u[0]);
             tmem_ld32_async(tO + 32, u[1]);
             tmem_ld_wait();
