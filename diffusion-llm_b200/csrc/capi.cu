@@ -1202,7 +1202,9 @@ constexpr int kPagedCtas = 2;  // CTAs an SM of paged_attn_kernel (paged_attn_tc
 // workers an SM at most
 constexpr int kPagedWorkers = bd3::kPtWorkers > kPagedCtas ? bd3::kPtWorkers : kPagedCtas;
 
-// Rows per sequence and KV head up to which paged_attn_kernel takes a call.
+// Rows per sequence and KV head up to which paged_attn_kernel takes a call, paged_attn_tc_kernel
+// above it. At 32 rows, 12 heads: 64 sequences of 332 positions 38 us against 39, one of 132
+// 10.0 against 11.6, two of 65568 88 against 85; at 64 rows of those two 165 against 85.
 constexpr int64_t kPagedMaxRows = 32;
 
 // Counts (zero between calls), then the partials of the widest kernel's row tile.

@@ -20,6 +20,13 @@
 // they were; then the CTA's threads take (token, row) pairs from the list, all lanes at work.
 // (Penalising them while streaming had one or two lanes of a warp divide at a time and took two
 // thirds of all instructions.)
+// Measured: 64 x 16 rows of 50258 bf16 logits with bias, mask and histories of 64 to 1024 tokens
+// 58 us (3.6 TB/s; 38 us without histories, where a copy takes 35: the scattered pass over the
+// listed tokens is the rest); 96 fp32 rows of 128001 with histories of up to 16384 59 us (2.5
+// TB/s; 34 us without histories: every slice's CTA scans all of a history, from L2). Slices of
+// 4096 and 8192 tokens, CTAs of 128, 512 and 1024 threads, 16-byte history loads, a table listed
+// by ballots and histories read by eighths in clusters of 8 CTAs (adding through distributed
+// shared memory) were all slower over these lengths.
 #pragma once
 
 #include "kv_rope.cuh"
