@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(kLogitThreads, 4) logits_kernel(const LogitPar
   const uint8_t* const in0 = reinterpret_cast<const uint8_t*>(p.logits) + b * p.l_sb * T::kBytes;
   uint8_t* const out0 = reinterpret_cast<uint8_t*>(p.out) + b * p.o_sb * T::kBytes;
   const uint32_t* const mask0 = p.allowed ? p.allowed + b * p.a_sb : nullptr;
-  const bool row_mask = mask0 != nullptr && p.a_ss != 0;
+  const bool row_mask = kR > 1 && mask0 != nullptr && p.a_ss != 0;  // (kR = 1: one row)
   const float* const bias = p.bias ? p.bias + b * p.bias_sb : nullptr;
   const int n_hist = p.history == nullptr ? 0 : max(0, min(p.hist_len[b], p.hist_cap));
   const float rep = p.repetition ? p.repetition[b] : 1.f;
@@ -137,20 +137,45 @@ __global__ void __launch_bounds__(kLogitThreads, 4) logits_kernel(const LogitPar
     return __funnelshift_r(m[v0 >> 5], m[(v0 + kE - 1) >> 5], v0 & 31) & kAll;
   };
 
+  // which bits of a chunk's four words the mask keeps
+  auto keep_of = [&](uint32_t ok, uint32_t (&keep)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (kDtype == 2) {
+        keep[j] = ok >> j & 1u ? 0xFFFFFFFFu : 0u;
+      } else {
+        const uint32_t two = ok >> (2 * j);
+        keep[j] = (two & 1u) * 0xFFFFu + (two & 2u) * 0x7FFF8000u;
+      }
+    }
+  };
+
   // rows of one alignment: s0 + c, s0 + c + period, ...
   const int step = static_cast<int>(p.l_ss & (kE - 1));
   const int period = step == 0 ? 1 : kE / (step & -step);
+  const long long step_in = period * p.l_ss * T::kBytes, step_out = period * p.o_ss * T::kBytes;
+  const bool same_step = ((step_in ^ step_out) & 15) == 0;  // in and out keep their distance mod 16
   bool counted = n_hist == 0;
   for (int c = 0; c < period && s0 + c < s1; ++c) {
     const int a = static_cast<int>(reinterpret_cast<uintptr_t>(in0 + (s0 + c) * p.l_ss * T::kBytes) / T::kBytes) & (kE - 1);
+    // of this thread's chunks in the rows of this alignment: first token, where the first row has
+    // it, its mask (0 at an end of the row or past it) and, as a 16-bit mask per logit, what to keep
     int v0[kU];
-    uint32_t ok_all[kU];
+    const uint8_t* pin[kU];
+    uint8_t* pout[kU];
+    uint32_t ok_all[kU], keep[kU][4];
     float bv[kU][kE];
+    const uint8_t* const in_c = in0 + (s0 + c) * p.l_ss * T::kBytes;
+    uint8_t* const out_c = out0 + (s0 + c) * p.o_ss * T::kBytes;
+    const bool vec = ((reinterpret_cast<uintptr_t>(in_c) ^ reinterpret_cast<uintptr_t>(out_c)) & 15) == 0 && same_step;
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
       v0[u] = (k0 + u * kLogitThreads + static_cast<int>(threadIdx.x)) * kE - a;
-      ok_all[u] = v0[u] >= 0 && v0[u] + kE <= p.V ? kAll : 0u;  // (0: an end of the row, or past it)
-      if (ok_all[u] != 0 && mask0 != nullptr && !row_mask) ok_all[u] = bits_of(mask0, v0[u]);
+      pin[u] = in_c + static_cast<long long>(v0[u]) * T::kBytes;
+      pout[u] = out_c + static_cast<long long>(v0[u]) * T::kBytes;
+      ok_all[u] = v0[u] >= 0 && v0[u] + kE <= p.V ? kAll : 0u;
+      if (ok_all[u] != 0 && mask0 != nullptr && !row_mask) ok_all[u] = bits_of(mask0 + s0 * p.a_ss, v0[u]);
+      keep_of(ok_all[u], keep[u]);
     }
     for (int sb = s0 + c; sb < s1; sb += period * kR) {
       uint32_t ok[kR][kU];
@@ -165,15 +190,10 @@ __global__ void __launch_bounds__(kLogitThreads, 4) logits_kernel(const LogitPar
         }
       }
 #pragma unroll
-      for (int r = 0; r < kR; ++r) {
-        const uint8_t* in = in0 + (sb + r * period) * p.l_ss * T::kBytes;
+      for (int r = 0; r < kR; ++r)
 #pragma unroll
-        for (int u = 0; u < kU; ++u) {
-          raw[r][u] = make_uint4(0, 0, 0, 0);
-          if (ok[r][u] != 0)
-            raw[r][u] = *reinterpret_cast<const uint4*>(in + static_cast<long long>(v0[u]) * T::kBytes);
-        }
-      }
+        for (int u = 0; u < kU; ++u)
+          if (ok[r][u] != 0) raw[r][u] = *reinterpret_cast<const uint4*>(pin[u] + r * step_in);
       if (sb == s0 + c) {  // once for the rows of this alignment, behind the first loads
         if (bias != nullptr) {
 #pragma unroll
@@ -201,7 +221,8 @@ __global__ void __launch_bounds__(kLogitThreads, 4) logits_kernel(const LogitPar
           for (int u = 0; u < kU; ++u) {
             if (ok_all[u] == 0) continue;
             const int x0 = v0[u] - base;
-            const uint32_t hit = __funnelshift_r(seen[x0 >> 5], seen[(x0 >> 5) + 1], x0 & 31);
+            const uint32_t hit = __funnelshift_r(seen[x0 >> 5], seen[(x0 >> 5) + 1], x0 & 31) & kAll;
+            if (hit == 0) continue;
 #pragma unroll
             for (int e = 0; e < kE; ++e)
               if (hit >> e & 1u) bv[u][e] = 0.f;
@@ -210,16 +231,11 @@ __global__ void __launch_bounds__(kLogitThreads, 4) logits_kernel(const LogitPar
       }
 #pragma unroll
       for (int r = 0; r < kR; ++r) {
-        const int s = sb + r * period;
-        if (s >= s1) break;
-        const uint8_t* in = in0 + s * p.l_ss * T::kBytes;
-        uint8_t* out = out0 + s * p.o_ss * T::kBytes;
-        const bool vec = ((reinterpret_cast<uintptr_t>(in) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+        if (sb + r * period >= s1) break;
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
           if (v0[u] < 0 || v0[u] + kE > p.V) continue;  // an end of the row, below, or past it
-          const uint4 x = raw[r][u];
-          uint32_t w[4] = {x.x, x.y, x.z, x.w};
+          uint32_t w[4] = {raw[r][u].x, raw[r][u].y, raw[r][u].z, raw[r][u].w};
           if (bias != nullptr) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -232,29 +248,27 @@ __global__ void __launch_bounds__(kLogitThreads, 4) logits_kernel(const LogitPar
             }
           }
           if (mask0 != nullptr) {  // forbidden tokens
+            constexpr uint32_t kInf = kDtype == 0 ? 0xFF80FF80u : kDtype == 1 ? 0xFC00FC00u : 0xFF800000u;
+            if (row_mask) keep_of(ok[r][u], keep[u]);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              if constexpr (kDtype == 2) {
-                if (!(ok[r][u] >> j & 1u)) w[j] = 0xFF800000u;
-              } else {
-                constexpr uint32_t kInf = kDtype == 0 ? 0xFF80FF80u : 0xFC00FC00u;
-                const uint32_t two = ok[r][u] >> (2 * j);
-                const uint32_t keep = (two & 1u) * 0xFFFFu + (two & 2u) * 0x7FFF8000u;
-                w[j] = (w[j] & keep) | (kInf & ~keep);
-              }
-            }
+            for (int j = 0; j < 4; ++j) w[j] = (w[j] & keep[u][j]) | (kInf & ~keep[u][j]);
           }
+          uint8_t* const out = pout[u] + r * step_out;
           if (vec) {
-            *reinterpret_cast<uint4*>(out + static_cast<long long>(v0[u]) * T::kBytes) =
-                make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(out) = make_uint4(w[0], w[1], w[2], w[3]);
           } else {
 #pragma unroll
             for (int e = 0; e < kE; ++e) {
-              if constexpr (kDtype == 2) reinterpret_cast<uint32_t*>(out)[v0[u] + e] = w[e];
-              else reinterpret_cast<uint16_t*>(out)[v0[u] + e] = static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1)));
+              if constexpr (kDtype == 2) reinterpret_cast<uint32_t*>(out)[e] = w[e];
+              else reinterpret_cast<uint16_t*>(out)[e] = static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1)));
             }
           }
         }
+      }
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        pin[u] += kR * step_in;
+        pout[u] += kR * step_out;
       }
     }
   }
