@@ -1426,7 +1426,7 @@ int launch_logits(bd3::LogitParams& p, int64_t B, int sms, void* stream) {
   if (p.S > 1) return launch_logits_u<kDtype, 1, 4>(p, B, sms, stream);
   constexpr int kSlice1 = bd3::LogitTile<kDtype, 1>::kSlice;
   const int64_t ctas = (p.V + kSlice1 - 1) / kSlice1 * B;  // at one chunk a thread
-  return ctas >= 8LL * sms ? launch_logits_u<kDtype, 2, 1>(p, B, sms, stream)
+  return ctas >= 8LL * sms ? launch_logits_u<kDtype, kDtype == 2 ? 4 : 2, 1>(p, B, sms, stream)
                            : launch_logits_u<kDtype, 1, 1>(p, B, sms, stream);
 }
 }  // namespace

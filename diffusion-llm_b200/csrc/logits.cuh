@@ -71,11 +71,10 @@ __device__ __forceinline__ float load_logit(const void* row, long long v) {
   else if constexpr (kDtype == 1) return __half2float(reinterpret_cast<const __half*>(row)[v]);
   else return reinterpret_cast<const float*>(row)[v];
 }
-// A value as the bits of its type.
 template <int kDtype>
-__device__ __forceinline__ uint32_t logit_bits(float x) {
-  if constexpr (kDtype == 2) return __float_as_uint(x);
-  else return pack2<kDtype == 0>(x, 0.f);  // the second value is in the high half: 0
+__device__ __forceinline__ void store_logit(void* row, long long v, float x) {
+  if constexpr (kDtype == 2) reinterpret_cast<float*>(row)[v] = x;
+  else reinterpret_cast<uint16_t*>(row)[v] = static_cast<uint16_t>(pack2<kDtype == 0>(x, x));
 }
 
 __device__ __forceinline__ float penalise(float x, float n, float rep, float freq, float pres) {
@@ -121,15 +120,17 @@ __global__ void __launch_bounds__(kLogitThreads, 4) logits_kernel(const LogitPar
         list[atomicAdd(&n_list, 1)] = static_cast<uint16_t>(x);
       }
     };
-    if (p.hist32) {
-      const int* h = reinterpret_cast<const int*>(p.history) + h0;
-#pragma unroll 4
-      for (int i = threadIdx.x; i < n_hist; i += kLogitThreads) add(h[i]);
-    } else {
-      const long long* h = reinterpret_cast<const long long*>(p.history) + h0;
-#pragma unroll 4
-      for (int i = threadIdx.x; i < n_hist; i += kLogitThreads) add(h[i]);
-    }
+    auto scan = [&](const auto* h) {  // 4 loads of a thread in flight
+      for (int i = threadIdx.x; i < n_hist; i += 4 * kLogitThreads) {
+        long long v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = i + j * kLogitThreads < n_hist ? h[i + j * kLogitThreads] : -1;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) add(v[j]);
+      }
+    };
+    if (p.hist32) scan(reinterpret_cast<const int*>(p.history) + h0);
+    else scan(reinterpret_cast<const long long*>(p.history) + h0);
     __syncthreads();
   };
   // the mask's bits of the tokens [v0, v0 + kE)
@@ -289,41 +290,70 @@ __global__ void __launch_bounds__(kLogitThreads, 4) logits_kernel(const LogitPar
       y = load_logit<kDtype>(in, v);
       if (bias != nullptr && !(n_hist > 0 && count[v - base] != 0)) y = __fadd_rn(y, bias[v]);
     }
-    uint8_t* out = out0 + s * p.o_ss * T::kBytes;
-    if constexpr (kDtype == 2) reinterpret_cast<float*>(out)[v] = y;
-    else reinterpret_cast<uint16_t*>(out)[v] = static_cast<uint16_t>(logit_bits<kDtype>(y));
+    store_logit<kDtype>(out0 + s * p.o_ss * T::kBytes, v, y);
   }
   if (n_hist == 0) return;
   // ---- the listed tokens ----
   __syncthreads();  // the rows are in `out`
-  const int pairs = n_list * (s1 - s0);
-  for (int i0 = threadIdx.x; i0 < pairs; i0 += 4 * kLogitThreads) {
-    int ps[4], px[4];
-    float y[4];
-    bool live[4];
+  if constexpr (kR == 1) {
+    // one row: a thread takes every kLogitThreads-th token, four loads at a time
+    for (int i0 = threadIdx.x; i0 < n_list; i0 += 4 * kLogitThreads) {
+      float y[4];
+      int px[4];
+      bool live[4];
+      const int a = static_cast<int>(reinterpret_cast<uintptr_t>(in0 + s0 * p.l_ss * T::kBytes) / T::kBytes) & (kE - 1);
+      uint8_t* const out = out0 + s0 * p.o_ss * T::kBytes;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = i0 + j * kLogitThreads;
-      live[j] = i < pairs;
-      if (!live[j]) continue;
-      const int r = i / n_list, s = s0 + r, x = list[i - r * n_list], v = base + x;
-      const int a = static_cast<int>(reinterpret_cast<uintptr_t>(in0 + s * p.l_ss * T::kBytes) / T::kBytes) & (kE - 1);
-      // not the neighbour's (the span's ends are, for some alignments), nor forbidden
-      live[j] = v >= k0 * kE - a && v < k0 * kE - a + T::kSlice &&
-                (mask0 == nullptr || (mask0[s * p.a_ss + (v >> 5)] >> (v & 31) & 1u));
-      ps[j] = s;
-      px[j] = x;
-      if (live[j]) y[j] = load_logit<kDtype>(out0 + s * p.o_ss * T::kBytes, v);
+      for (int j = 0; j < 4; ++j) {
+        const int i = i0 + j * kLogitThreads;
+        live[j] = i < n_list;
+        if (!live[j]) continue;
+        px[j] = list[i];
+        const int v = base + px[j];
+        // not the neighbour's (the span's ends are, for some alignments), nor forbidden
+        live[j] = v >= k0 * kE - a && v < k0 * kE - a + T::kSlice &&
+                  (mask0 == nullptr || (mask0[s0 * p.a_ss + (v >> 5)] >> (v & 31) & 1u));
+        if (live[j]) y[j] = load_logit<kDtype>(out, v);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (!live[j]) continue;
+        const int v = base + px[j];
+        y[j] = penalise(y[j], static_cast<float>(count[px[j]]), rep, freq, pres);
+        if (bias != nullptr) y[j] = __fadd_rn(y[j], bias[v]);
+        store_logit<kDtype>(out, v, y[j]);
+      }
     }
+    return;
+  }
+  // a thread takes a token and every `groups`-th row: its count, bias and shared mask once
+  const int rows = s1 - s0, listed = n_list;
+  const int groups = listed == 0 ? 1 : min(rows, max(1, kLogitThreads / listed));
+  for (int i = threadIdx.x; i < listed * groups; i += kLogitThreads) {
+    const int g = i / listed, x = list[i - g * listed], v = base + x;
+    const float n = static_cast<float>(count[x]), bias_v = bias != nullptr ? bias[v] : 0.f;
+    if (mask0 != nullptr && !row_mask && !(mask0[s0 * p.a_ss + (v >> 5)] >> (v & 31) & 1u)) continue;
+    for (int r = g; r < rows; r += 4 * groups) {
+      float y[4];
+      bool live[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (!live[j]) continue;
-      const int v = base + px[j];
-      y[j] = penalise(y[j], static_cast<float>(count[px[j]]), rep, freq, pres);
-      if (bias != nullptr) y[j] = __fadd_rn(y[j], bias[v]);
-      uint8_t* out = out0 + ps[j] * p.o_ss * T::kBytes;
-      if constexpr (kDtype == 2) reinterpret_cast<float*>(out)[v] = y[j];
-      else reinterpret_cast<uint16_t*>(out)[v] = static_cast<uint16_t>(logit_bits<kDtype>(y[j]));
+      for (int j = 0; j < 4; ++j) {
+        const int s = s0 + r + j * groups;
+        live[j] = s < s1;
+        if (!live[j]) continue;
+        // not the neighbour's (the span's ends are, for some alignments), nor forbidden
+        const int a = static_cast<int>(reinterpret_cast<uintptr_t>(in0 + s * p.l_ss * T::kBytes) / T::kBytes) & (kE - 1);
+        live[j] = v >= k0 * kE - a && v < k0 * kE - a + T::kSlice &&
+                  (!row_mask || (mask0[s * p.a_ss + (v >> 5)] >> (v & 31) & 1u));
+        if (live[j]) y[j] = load_logit<kDtype>(out0 + s * p.o_ss * T::kBytes, v);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (!live[j]) continue;
+        y[j] = penalise(y[j], n, rep, freq, pres);
+        if (bias != nullptr) y[j] = __fadd_rn(y[j], bias_v);
+        store_logit<kDtype>(out0 + (s0 + r + j * groups) * p.o_ss * T::kBytes, v, y[j]);
+      }
     }
   }
 }
