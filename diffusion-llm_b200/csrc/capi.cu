@@ -1421,6 +1421,9 @@ int launch_logits_u(bd3::LogitParams& p, int64_t B, int sms, void* stream) {
                     dim3(bd3::kLogitThreads), 0, static_cast<cudaStream_t>(stream),
                     "logits_kernel launch", p);
 }
+// Several rows: four of one alignment at a time. One row: 4096 tokens a CTA where that leaves four
+// CTAs an SM (fewer CTAs scan the history: 96 rows of 128001 fp32 with 1024 tokens each 35 us
+// against 38 at 2048), else one chunk a thread (one row of 50258 bf16: 2.3 us against 2.7).
 template <int kDtype>
 int launch_logits(bd3::LogitParams& p, int64_t B, int sms, void* stream) {
   if (p.S > 1) return launch_logits_u<kDtype, 1, 4>(p, B, sms, stream);

@@ -8,24 +8,24 @@
 // logits' type. The S rows of a sequence (a block of a denoising step) share its history.
 //
 // DRAM-bound: every logit is read and written once, 16 bytes an access; a chunk of eight (four in
-// fp32) tokens that the mask forbids is not read. The streaming has 25 to 30 cycles of an SM
-// sub-partition for 32 chunks, so what is the same for several rows is worked out once. A CTA
-// takes a slice of the vocabulary, kU chunks a thread, for some rows of one sequence. Rows of an
-// odd vocabulary start at any alignment, so a row's chunks begin `a` logits before the
-// multiples of the chunk, a being its misalignment, which repeats every `period` rows: the CTA
-// takes the rows of one alignment together, with their mask, bias and hits of the history in
-// registers, kR rows' loads at a time. (The two ends of a row go one logit at a time.)
+// fp32) tokens that the mask forbids is not read. At that rate a warp has about 170 issue slots
+// for 32 chunks, so what is the same for several rows is worked out once. A CTA takes a slice of
+// the vocabulary, kU chunks a thread, for some rows of one sequence. Rows of an odd vocabulary
+// start at any alignment, so a row's chunks begin `a` logits before the multiples of the chunk,
+// a being its misalignment, which repeats every `period` rows: the CTA takes the rows of one
+// alignment together, with their mask and bias in registers, kR rows' loads at a time. (The two
+// ends of a row go one logit a thread.)
 // The history's tokens of the slice are counted in shared memory behind the first loads (integer
 // atomics: their order does not matter) and listed. The streaming leaves the listed tokens as
-// they were; then the CTA's threads take (token, row) pairs from the list, all lanes at work.
-// (Penalising them while streaming had one or two lanes of a warp divide at a time and took two
-// thirds of all instructions.)
+// they were; then the CTA's threads go over the list, all lanes at work. (Penalising them while
+// streaming had one or two lanes of a warp divide at a time and took two thirds of all
+// instructions.)
 // Measured: 64 x 16 rows of 50258 bf16 logits with bias, mask and histories of 64 to 1024 tokens
-// 58 us (3.6 TB/s; 38 us without histories, where a copy takes 35: the scattered pass over the
-// listed tokens is the rest); 96 fp32 rows of 128001 with histories of up to 16384 59 us (2.5
-// TB/s; 34 us without histories: every slice's CTA scans all of a history, from L2). Slices of
-// 4096 and 8192 tokens, CTAs of 128, 512 and 1024 threads, 16-byte history loads, a table listed
-// by ballots and histories read by eighths in clusters of 8 CTAs (adding through distributed
+// 53 us (41 us without histories, where a copy takes 35; the scattered pass over the listed
+// tokens is the rest); 96 fp32 rows of 128001 with histories of up to 16384 55 us (33 us without:
+// every slice's CTA scans all of its sequence's history, from L2). Slices of 8192 tokens, CTAs of
+// 128, 512 and 1024 threads, eight or more history loads in flight, a list made by ballots over
+// the counts, and histories read by eighths in clusters of 8 CTAs (adding through distributed
 // shared memory) were all slower over these lengths.
 #pragma once
 
