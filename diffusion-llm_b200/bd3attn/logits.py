@@ -14,15 +14,15 @@ import ctypes
 import torch
 
 from bd3attn._lib import LIB, check
-from bd3attn.ops import _check_cuda, _code, _raw_stream
+from bd3attn.ops import _check_cuda, _check_on, _code, _raw_stream
 
 _I64x2, _I64x4 = ctypes.c_int64 * 2, ctypes.c_int64 * 4
 
 
-def _per_sequence(name, t, B):
+def _per_sequence(name, t, B, index):
     if t is None:
         return None
-    _check_cuda(t)
+    _check_on(index, t)
     if t.dtype != torch.float32 or t.shape != (B,) or not t.is_contiguous():
         raise AssertionError(f"{name} must be a contiguous (batch,) fp32 tensor")
     return t.data_ptr()
@@ -75,7 +75,7 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None,
     if history is not None:
         if history_len is None:
             raise AssertionError("history needs history_len")
-        _check_cuda(history, history_len)
+        _check_on(dev.index, history, history_len)
         if history.dtype not in (torch.int64, torch.int32) or history.dim() != 2 \
                 or history.shape[0] != B or (history.stride(1) != 1 and history.shape[1] > 1):
             raise AssertionError("history must be (batch, capacity) int64 or int32 tokens")
@@ -87,14 +87,14 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None,
             history.shape[1]
     b_ptr, b_stride = None, 0
     if bias is not None:
-        _check_cuda(bias)
+        _check_on(dev.index, bias)
         if bias.dtype != torch.float32 or bias.shape not in ((V,), (B, V)) \
                 or (bias.stride(-1) != 1 and V > 1):
             raise AssertionError("bias must be (vocab,) or (batch, vocab) fp32")
         b_ptr, b_stride = bias.data_ptr(), bias.stride(0) if bias.dim() == 2 else 0
     a_ptr = a_strides = None
     if allowed is not None:
-        _check_cuda(allowed)
+        _check_on(dev.index, allowed)
         words = (V + 31) // 32
         if allowed.dtype != torch.int32 or allowed.shape not in ((B, words), (B, S, words)) \
                 or (allowed.stride(-1) != 1 and words > 1):
@@ -106,9 +106,11 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None,
     rc = LIB.bd3_process_logits(
         logits.data_ptr(), out.data_ptr(),
         _I64x4(logits.stride(0), logits.stride(1), out.stride(0), out.stride(1)), B, S, V,
-        h_ptr, h_i32, h_stride, h_cap, hl_ptr, _per_sequence("repetition", repetition, B),
-        _per_sequence("presence", presence, B), _per_sequence("frequency", frequency, B), b_ptr,
-        b_stride, a_ptr, a_strides, _code(logits.dtype), _raw_stream(dev))
+        h_ptr, h_i32, h_stride, h_cap, hl_ptr,
+        _per_sequence("repetition", repetition, B, dev.index),
+        _per_sequence("presence", presence, B, dev.index),
+        _per_sequence("frequency", frequency, B, dev.index), b_ptr, b_stride, a_ptr, a_strides,
+        _code(logits.dtype), _raw_stream(dev))
     if rc:
         check("bd3_process_logits", rc)
     return out

@@ -383,12 +383,18 @@ def _(qkv, n_heads, cos_table, sin_table, k_cache, v_cache, row0, positions=None
 _I64x9, _I64x11 = ctypes.c_int64 * 9, ctypes.c_int64 * 11
 
 
+def _check_on(index: int, *xs) -> None:
+    """All on the CUDA device of that index (get_device() is -1 on the CPU)."""
+    for x in xs:
+        if x.get_device() != index:
+            raise AssertionError("all tensors must be on the same CUDA device")
+
+
 def _raw_stream(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _check_pages(k_pages, v_pages, page_table, kv_lens, cu_q, dtype, n_kv_heads, D):
-    _check_cuda(k_pages, v_pages, page_table, kv_lens, cu_q)
     ks = k_pages.shape
     if len(ks) != 4 or ks != v_pages.shape or ks[1] != n_kv_heads or ks[3] != D:
         raise AssertionError("k_pages and v_pages must be (pages, kv heads, page size, head_dim)")
@@ -432,6 +438,7 @@ def paged_attn_raw(q, k_pages, v_pages, page_table, kv_lens, cu_q, max_q_len: in
     tokens of a sequence. Tensors of lengths stay on the device: a captured CUDA graph serves
     other lengths and tables. workspace: paged_workspace(), kept by the caller (None: a new
     zeroed one). Returns O (tokens, q heads, 64), with the LSE (tokens, q heads) if asked.
+    Forward only, as the other decode functions.
     """
     _check_cuda(q)
     dev = q.device
@@ -449,6 +456,7 @@ def paged_attn_raw(q, k_pages, v_pages, page_table, kv_lens, cu_q, max_q_len: in
         q = q.clone(memory_format=torch.contiguous_format)
         qs = q.stride()
     code = _code(q.dtype)
+    _check_on(dev.index, k_pages, v_pages, page_table, kv_lens, cu_q)
     if out_dtype is None or out_dtype == q.dtype:
         o, out_code = torch.empty_like(q, memory_format=torch.contiguous_format), code
     else:
@@ -481,7 +489,7 @@ def qkv_rope_paged_raw(qkv, n_heads: int, n_kv_heads: int, cos_table, sin_table,
     sin_table: (max_pos, D / 2) fp32; the rest as paged_attn_raw (kv_lens counts the tokens
     being written). The rotation is fp32, rounded once.
     """
-    _check_cuda(qkv, cos_table, sin_table)
+    _check_cuda(qkv)
     dev = qkv.device
     if torch.cuda.current_device() != dev.index:
         with torch.cuda.device(dev):
@@ -499,6 +507,7 @@ def qkv_rope_paged_raw(qkv, n_heads: int, n_kv_heads: int, cos_table, sin_table,
         raise AssertionError("cos_table and sin_table must be contiguous (max_pos, head_dim / 2) fp32")
     if qkv.stride(1) != 1 or qkv.stride(0) * qkv.element_size() % 16 or qkv.data_ptr() % 16:
         qkv = qkv.clone(memory_format=torch.contiguous_format)
+    _check_on(dev.index, cos_table, sin_table, k_pages, v_pages, page_table, kv_lens, cu_q)
     if q_out is None:
         q_out = qkv.new_empty((T, n_heads, D))
     elif q_out.shape != (T, n_heads, D) or q_out.dtype != qkv.dtype or q_out.stride(2) != 1 \
