@@ -56,7 +56,7 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None,
     """
     _check_cuda(logits)
     dev = logits.device
-    if torch.cuda.current_device() != dev.index:
+    if torch._C._cuda_getDevice() != dev.index:
         with torch.cuda.device(dev):
             return process_logits(logits, history, history_len, repetition, presence, frequency,
                                   bias, allowed, out)

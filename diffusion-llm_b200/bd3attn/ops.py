@@ -398,20 +398,20 @@ def _check_pages(k_pages, v_pages, page_table, kv_lens, cu_q, dtype, n_kv_heads,
     ks = k_pages.shape
     if len(ks) != 4 or ks != v_pages.shape or ks[1] != n_kv_heads or ks[3] != D:
         raise AssertionError("k_pages and v_pages must be (pages, kv heads, page size, head_dim)")
-    if k_pages.dtype != dtype or v_pages.dtype != dtype:
+    if k_pages.dtype is not dtype or v_pages.dtype is not dtype:
         raise AssertionError("k_pages and v_pages must be in the new tokens' dtype")
-    if page_table.dtype != torch.int32 or kv_lens.dtype != torch.int32 \
-            or cu_q.dtype != torch.int32:
+    i32 = torch.int32
+    if page_table.dtype is not i32 or kv_lens.dtype is not i32 or cu_q.dtype is not i32:
         raise AssertionError("page_table, kv_lens and cu_q must be int32")
-    B = kv_lens.shape[0] if kv_lens.dim() == 1 else -1
-    if page_table.dim() != 2 or page_table.shape[0] != B or cu_q.shape != (B + 1,) \
-            or not cu_q.is_contiguous() or not kv_lens.is_contiguous() \
-            or (page_table.stride(1) != 1 and page_table.shape[1] > 1):
+    ts, bs, cs = page_table.shape, kv_lens.shape, cu_q.shape
+    if len(ts) != 2 or len(bs) != 1 or len(cs) != 1 or ts[0] != bs[0] or cs[0] != bs[0] + 1 \
+            or not kv_lens.is_contiguous() or not cu_q.is_contiguous() \
+            or (page_table.stride(1) != 1 and ts[1] > 1):
         raise AssertionError("page_table must be (B, pages), kv_lens (B,) and cu_q (B + 1,)")
     kst, vst = k_pages.stride(), v_pages.stride()
     if kst[3] != 1 or vst[3] != 1:
         raise AssertionError("the pages' head_dim must be contiguous")
-    return B, kst, vst
+    return bs[0], ts[1], kst, vst
 
 
 def paged_workspace(device=None) -> torch.Tensor:
@@ -442,7 +442,7 @@ def paged_attn_raw(q, k_pages, v_pages, page_table, kv_lens, cu_q, max_q_len: in
     """
     _check_cuda(q)
     dev = q.device
-    if torch.cuda.current_device() != dev.index:
+    if torch._C._cuda_getDevice() != dev.index:
         with torch.cuda.device(dev):
             return paged_attn_raw(q, k_pages, v_pages, page_table, kv_lens, cu_q, max_q_len,
                                   block_size, scale, out_dtype, return_lse, workspace)
@@ -450,7 +450,7 @@ def paged_attn_raw(q, k_pages, v_pages, page_table, kv_lens, cu_q, max_q_len: in
         raise AssertionError("q must be (tokens, q heads, head_dim)")
     T, Hq, D = q.shape
     n_pages, Hkv, page_size = k_pages.shape[:3] if k_pages.dim() == 4 else (0, 0, 0)
-    B, ks, vs = _check_pages(k_pages, v_pages, page_table, kv_lens, cu_q, q.dtype, Hkv, D)
+    B, width, ks, vs = _check_pages(k_pages, v_pages, page_table, kv_lens, cu_q, q.dtype, Hkv, D)
     qs = q.stride()
     if qs[2] != 1 or qs[0] % 8 or qs[1] % 8 or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
@@ -469,8 +469,7 @@ def paged_attn_raw(q, k_pages, v_pages, page_table, kv_lens, cu_q, max_q_len: in
     rc = LIB.bd3_paged_attn(
         q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), o.data_ptr(),
         lse.data_ptr() if return_lse else None, page_table.data_ptr(), kv_lens.data_ptr(),
-        cu_q.data_ptr(), B, T, int(max_q_len), Hq, Hkv, D, n_pages, page_size,
-        page_table.shape[1],
+        cu_q.data_ptr(), B, T, int(max_q_len), Hq, Hkv, D, n_pages, page_size, width,
         _I64x11(qs[0], qs[1], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], Hq * D, D,
                 page_table.stride(0)),
         int(block_size), D ** -0.5 if scale is None else float(scale), code, out_code,
@@ -491,7 +490,7 @@ def qkv_rope_paged_raw(qkv, n_heads: int, n_kv_heads: int, cos_table, sin_table,
     """
     _check_cuda(qkv)
     dev = qkv.device
-    if torch.cuda.current_device() != dev.index:
+    if torch._C._cuda_getDevice() != dev.index:
         with torch.cuda.device(dev):
             return qkv_rope_paged_raw(qkv, n_heads, n_kv_heads, cos_table, sin_table, k_pages,
                                       v_pages, page_table, kv_lens, cu_q, q_out)
@@ -500,7 +499,7 @@ def qkv_rope_paged_raw(qkv, n_heads: int, n_kv_heads: int, cos_table, sin_table,
         raise AssertionError("qkv must be (tokens, (n_heads + 2 * n_kv_heads) * head_dim)")
     T, F = qkv.shape
     D = F // heads
-    B, ks, vs = _check_pages(k_pages, v_pages, page_table, kv_lens, cu_q, qkv.dtype, n_kv_heads, D)
+    B, width, ks, vs = _check_pages(k_pages, v_pages, page_table, kv_lens, cu_q, qkv.dtype, n_kv_heads, D)
     if cos_table.dtype != torch.float32 or sin_table.dtype != torch.float32 \
             or cos_table.shape != sin_table.shape or cos_table.shape[1:] != (D // 2,) \
             or not cos_table.is_contiguous() or not sin_table.is_contiguous():
@@ -517,7 +516,7 @@ def qkv_rope_paged_raw(qkv, n_heads: int, n_kv_heads: int, cos_table, sin_table,
         qkv.data_ptr(), qkv.stride(0), T, B, n_heads, n_kv_heads, D, cos_table.data_ptr(),
         sin_table.data_ptr(), cos_table.shape[0], q_out.data_ptr(), k_pages.data_ptr(),
         v_pages.data_ptr(), page_table.data_ptr(), kv_lens.data_ptr(), cu_q.data_ptr(),
-        k_pages.shape[0], k_pages.shape[2], page_table.shape[1],
+        k_pages.shape[0], k_pages.shape[2], width,
         _I64x9(q_out.stride(0), q_out.stride(1), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
                page_table.stride(0)),
         _code(qkv.dtype), _raw_stream(dev))
