@@ -68,6 +68,7 @@ SIGNATURES = {
                            [_vp] * 5 + [_i64, _vp, _pi64, _i32, _vp]),
     "bd3_profile_enable": (_i32, [_i32]),
     "bd3_profile_collect": (_i32, [ctypes.POINTER(ctypes.c_double), _pi32]),
+    "bd3_profile_collect_all": (_i32, [ctypes.POINTER(ctypes.c_double), _pi32, _i32]),
     "bd3_debug_ranges": (_i32, [_i32, _i64, _i64, _i64, _i64, _i64, _i64, _pi32]),
     "bd3_debug_tiles": (_i32, [_pi32]),
     "bd3_debug_wait_timeout": (_i32, [_i64, _i32, _vp, _vp]),

@@ -556,7 +556,8 @@ def _(qkv, n_heads, n_kv_heads, cos_table, sin_table, k_pages, v_pages, page_tab
 
 # ---------------------------------------------------------------------------------------
 PROFILE_KERNELS = ("attn_fwd", "attn_prefill", "bwd_prep", "bwd_dq_convert", "bwd_fused",
-                   "decode", "decode_combine", "qkv_rope_cache", "subs_sample")
+                   "decode", "decode_combine", "qkv_rope_cache", "subs_sample", "paged_attn",
+                   "qkv_rope_paged", "process_logits")
 
 
 def profile_enable(on: bool = True) -> None:
@@ -569,7 +570,7 @@ def profile_collect() -> dict:
     """{kernel name: (total ms, launches)} for the launches since the last collect."""
     ms = (ctypes.c_double * 16)()
     cnt = (ctypes.c_int32 * 16)()
-    n = LIB.bd3_profile_collect(ms, cnt)
+    n = LIB.bd3_profile_collect_all(ms, cnt, len(PROFILE_KERNELS))
     if n < 0:
         check("bd3_profile_collect", -n)
     return {PROFILE_KERNELS[i]: (ms[i], cnt[i]) for i in range(len(PROFILE_KERNELS)) if cnt[i]}

@@ -138,7 +138,8 @@ int set_smem(K kernel, uint32_t bytes, int slot) {
 // ---- optional per-kernel timing (bd3_profile_*): CUDA event pairs around each launch ----
 enum ProfId {
   kPfFwd = 0, kPfPrefill, kPfDelta, kPfDq, kPfDkdv, kPfDecode, kPfCombine, kPfRope, kPfSample,
-  kPfNum
+  kPfNum9,  // those of bd3_profile_collect
+  kPfPaged = kPfNum9, kPfPagedRope, kPfLogits, kPfNum
 };
 constexpr int kProfCap = 8192;
 struct Prof {
@@ -1261,7 +1262,7 @@ int bd3_paged_attn(const void* q, const void* k_pages, const void* v_pages, void
   if (workspace == nullptr) return fail(BD3_ERR_WORKSPACE, "paged attention needs its workspace");
   int sms = 148;
   if ((rc = ensure_context()) != BD3_OK || (rc = current_device_sms(&sms)) != BD3_OK) return rc;
-  if ( reinterpret_cast<uintptr_t>(workspace) % 16 ||
+  if (reinterpret_cast<uintptr_t>(workspace) % 16 ||
       workspace_bytes < paged_workspace_bytes(sms))
     return fail(BD3_ERR_WORKSPACE, "paged attention workspace: need %zu bytes, zeroed once",
                 paged_workspace_bytes(sms));
@@ -1329,6 +1330,7 @@ int bd3_paged_attn(const void* q, const void* k_pages, const void* v_pages, void
     if (n != bd3::kPtRegs)
       return fail(BD3_ERR_CUDA, "paged attention was built with %d registers a thread, not %d", n, bd3::kPtRegs);
   }
+  ProfScope ps(kPfPaged, static_cast<cudaStream_t>(stream));
   return launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(threads), smem,
                     static_cast<cudaStream_t>(stream), "paged attention launch", tk, tv, p);
 }
@@ -1398,6 +1400,7 @@ int bd3_qkv_rope_paged(const void* qkv, int64_t qkv_stride, int64_t T, int64_t B
               : dtype == BD3_F16 ? bd3::qkv_rope_paged_kernel<1>
                                  : bd3::qkv_rope_paged_kernel<2>;
   const int64_t grid = (T + p.tpb - 1) / p.tpb;
+  ProfScope ps(kPfPagedRope, static_cast<cudaStream_t>(stream));
   return launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(256), 0,
                     static_cast<cudaStream_t>(stream), "qkv_rope_paged_kernel launch", p);
 }
@@ -1416,6 +1419,7 @@ int launch_logits_u(bd3::LogitParams& p, int64_t B, int sms, void* stream) {
   const int64_t z = (p.S + rows - 1) / rows;
   if (z > 65535) return fail(BD3_ERR_UNSUPPORTED, "too many rows");
   p.rows = static_cast<int>(rows);
+  ProfScope ps(kPfLogits, static_cast<cudaStream_t>(stream));
   return launch_pdl(bd3::logits_kernel<kDtype, kU, kR>,
                     dim3(static_cast<unsigned>(slices), static_cast<unsigned>(B), static_cast<unsigned>(z)),
                     dim3(bd3::kLogitThreads), 0, static_cast<cudaStream_t>(stream),
@@ -1456,6 +1460,11 @@ int bd3_process_logits(const void* logits, void* out, const int64_t* strides, in
     return fail(BD3_ERR_INVALID, "history needs its lengths (int32) and at most 2^30 entries");
   if (allowed != nullptr && allowed_strides == nullptr)
     return fail(BD3_ERR_INVALID, "allowed needs its strides");
+  for (const void* x : {static_cast<const void*>(history_len), static_cast<const void*>(repetition),
+                        static_cast<const void*>(presence), static_cast<const void*>(frequency),
+                        static_cast<const void*>(bias), static_cast<const void*>(allowed)})
+    if (reinterpret_cast<uintptr_t>(x) % 4)
+      return fail(BD3_ERR_INVALID, "lengths, penalties, bias and mask must be 4-byte aligned");
   int rc, sms = 148;
   if ((rc = ensure_context()) != BD3_OK || (rc = current_device_sms(&sms)) != BD3_OK) return rc;
   bd3::LogitParams p{};
@@ -1502,23 +1511,30 @@ int bd3_profile_enable(int on) {
   return BD3_OK;
 }
 
-int bd3_profile_collect(double* total_ms, int32_t* counts) {
+int bd3_profile_collect_all(double* total_ms, int32_t* counts, int cap) {
   Prof& p = prof();
-  for (int k = 0; k < kPfNum; ++k) {
+  const int num = cap < 0 ? 0 : cap < kPfNum ? cap : kPfNum;
+  for (int k = 0; k < num; ++k) {
     total_ms[k] = 0.0;
     counts[k] = 0;
   }
   for (int i = 0; i < p.n; ++i) {
     cudaError_t e = cudaEventSynchronize(p.ev[i][1]);
-    if (e != cudaSuccess) return cuda_fail(e, "cudaEventSynchronize");
+    if (e != cudaSuccess) return -cuda_fail(e, "cudaEventSynchronize");
+    if (p.id[i] >= num) continue;
     float ms = 0.f;
     e = cudaEventElapsedTime(&ms, p.ev[i][0], p.ev[i][1]);
-    if (e != cudaSuccess) return cuda_fail(e, "cudaEventElapsedTime");
+    if (e != cudaSuccess) return -cuda_fail(e, "cudaEventElapsedTime");
     total_ms[p.id[i]] += ms;
     counts[p.id[i]] += 1;
   }
   p.n = 0;
-  return kPfNum;
+  return num;
+}
+
+int bd3_profile_collect(double* total_ms, int32_t* counts) {
+  const int n = bd3_profile_collect_all(total_ms, counts, kPfNum9);
+  return n < 0 ? -n : n;
 }
 
 int bd3_debug_ranges(int kind, int64_t start, int64_t tile_a, int64_t tile_b, int64_t n_or_qlen,

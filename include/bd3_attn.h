@@ -365,9 +365,13 @@ BD3_API int bd3_process_logits(const void* logits, void* out, const int64_t* str
  * 8 sampler step), the summed milliseconds
  * and launch counts to
  * total_ms[9] and counts[9]; it returns 9 and forgets the recorded launches.
+ * bd3_profile_collect_all() does so for the first `cap` ids, those of the serving kernels among
+ * them (9 paged attention, 10 QKV RoPE page write, 11 logits), and returns how many it
+ * wrote, or minus an error code.
  */
 BD3_API int bd3_profile_enable(int on);
 BD3_API int bd3_profile_collect(double* total_ms, int32_t* counts);
+BD3_API int bd3_profile_collect_all(double* total_ms, int32_t* counts, int cap);
 
 /* ---------------------------------------------------------------------------------------
  * Host-only introspection for tests (no GPU needed).

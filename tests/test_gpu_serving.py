@@ -91,6 +91,28 @@ def test_penalties_reach_the_draw(model):
     assert any((o < 240).any() for o in free) and not any((o < 240).any() for o in held)
 
 
+def test_the_timing_hooks_count_the_serving_launches():
+    """A page write, an attention (each of its kernels) and a logits call under the timing hooks."""
+    from bd3attn import ops
+    from bd3attn.logits import process_logits
+    tab = torch.ones(64, 32, device="cuda")
+    kp, vp = (torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    pages = torch.arange(4, dtype=torch.int32, device="cuda").view(1, 4)
+    lens, cu = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([40], [0, 40]))
+    qkv = torch.randn(40, 8 * 64, device="cuda").bfloat16()
+    ops.profile_enable(True)
+    try:
+        q = ops.qkv_rope_paged_raw(qkv, 4, 2, tab, tab, kp, vp, pages, lens, cu)
+        ops.paged_attn_raw(q, kp, vp, pages, lens, cu // 4, 10, 16)
+        ops.paged_attn_raw(q, kp, vp, pages, lens, cu, 40, 16)
+        process_logits(torch.randn(2, 3, 100, device="cuda"))
+        got = {k: n for k, (ms, n) in ops.profile_collect().items() if ms > 0}
+    finally:
+        ops.profile_enable(False)
+    assert_device_ok()
+    assert got == {"qkv_rope_paged": 1, "paged_attn": 2, "process_logits": 1}
+
+
 def test_a_captured_step_serves_growing_sequences(model):
     """One denoising forward captured in a CUDA graph, replayed block after block as begin()
     advances the lengths and hands out pages."""

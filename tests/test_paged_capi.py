@@ -80,6 +80,15 @@ def test_logits_refusals():
         assert _logits(**over) == BD3_ERR_UNSUPPORTED, over
 
 
+def test_logits_refuse_misaligned_vectors():
+    from bd3attn._lib import BD3_ERR_INVALID, LIB, i64_array
+    fine = [0x4000] * 6  # lengths, repetition, presence, frequency, bias, mask
+    for i in range(6):
+        a = fine[:i] + [0x4000 + 1 + i % 3] + fine[i + 1:]
+        assert LIB.bd3_process_logits(0x1000, 0x2000, i64_array([300, 100] * 2), 2, 3, 100, 0x3000, 0, 8, 8,
+                                      *a[:5], 0, a[5], i64_array([4, 0]), 0, None) == BD3_ERR_INVALID, i
+
+
 def test_oracle_attention_on_a_contiguous_cache():
     """Pages in order: the paged oracle equals the block-causal oracle of the contiguous cache."""
     import oracle
