@@ -1425,12 +1425,14 @@ int launch_logits_u(bd3::LogitParams& p, int64_t B, int sms, void* stream) {
                     dim3(bd3::kLogitThreads), 0, static_cast<cudaStream_t>(stream),
                     "logits_kernel launch", p);
 }
-// Several rows: four of one alignment at a time. One row: 4096 tokens a CTA where that leaves four
-// CTAs an SM (fewer CTAs scan the history: 96 rows of 128001 fp32 with 1024 tokens each 35 us
-// against 38 at 2048), else one chunk a thread (one row of 50258 bf16: 2.3 us against 2.7).
+// Several rows: two of one alignment at a time (four leave five CTAs an SM: 32 x 8 rows of 50257
+// fp32 31 us against 28, 8 x 16 of 50258 bf16 16.5 against 14.2). One row: 4096 tokens a CTA where
+// that leaves four CTAs an SM (fewer CTAs scan the history: 96 fp32 rows of 128001 with 16384
+// tokens each 81 us against 93 at 2048, with 1024 each 40 against 38.5), else one chunk a thread
+// (one row of 50258 bf16: 2.3 us against 2.7).
 template <int kDtype>
 int launch_logits(bd3::LogitParams& p, int64_t B, int sms, void* stream) {
-  if (p.S > 1) return launch_logits_u<kDtype, 1, 4>(p, B, sms, stream);
+  if (p.S > 1) return launch_logits_u<kDtype, 1, 2>(p, B, sms, stream);
   constexpr int kSlice1 = bd3::LogitTile<kDtype, 1>::kSlice;
   const int64_t ctas = (p.V + kSlice1 - 1) / kSlice1 * B;  // at one chunk a thread
   return ctas >= 8LL * sms ? launch_logits_u<kDtype, kDtype == 2 ? 4 : 2, 1>(p, B, sms, stream)

@@ -15,19 +15,23 @@
 // a being its misalignment, which repeats every `period` rows: the CTA takes the rows of one
 // alignment together, with their mask and bias in registers, kR rows' loads at a time. (The two
 // ends of a row go one logit a thread.)
-// The history's tokens of the slice are counted in shared memory behind the first loads (integer
-// atomics: their order does not matter) and listed. The streaming leaves the listed tokens as
-// they were; then the CTA's threads go over the list, all lanes at work. (Penalising them while
-// streaming had one or two lanes of a warp divide at a time and took two thirds of all
-// instructions.)
+// The history's tokens of the slice are counted in shared memory (integer atomics: their order
+// does not matter) and listed. The streaming leaves the listed tokens as they were; then the CTA's
+// threads go over the list, all lanes at work. (Penalising them while streaming has one or two
+// lanes of a warp divide at a time: two thirds of all instructions with several rows; single fp32
+// rows do it all the same, see kInline.)
 // Measured: 64 x 16 rows of 50258 bf16 logits with bias, mask and histories of 64 to 1024 tokens
-// 53 us (41 us without histories, where a copy takes 35; the scattered pass over the listed
-// tokens is the rest); 96 fp32 rows of 128001 with histories of up to 16384 55 us (33 us without:
-// every slice's CTA scans all of its sequence's history, from L2). Slices of 8192 tokens, CTAs of
-// 128, 512 and 1024 threads, eight or more history loads in flight, a list made by ballots over
-// the counts, and histories read by eighths in clusters of 8 CTAs (adding through distributed
-// shared memory) were all slower over these lengths.
+// 50 us (42 us with histories up to 64, where a copy takes 35; the scattered pass over the listed
+// tokens is the rest); 96 fp32 rows of 128001 44 us with histories of up to 16384 (1296 in the
+// mean), 38 with up to 64, 81 with 16384 each: every slice's CTA scans all of its sequence's
+// history, from L2. Before, with the counting behind the logits' loads at four CTAs an SM and four
+// rows at a time, those took 53, 46, 55, 40 and 129 us. Slices of 8192 tokens, CTAs of 128, 512 and
+// 1024 threads, eight or more history loads in flight, the next batch loaded ahead (70 against 55),
+// a list made by ballots over the counts, and histories read by eighths in clusters of 8 CTAs
+// (adding through distributed shared memory) were all slower over these lengths.
 #pragma once
+
+#include <type_traits>
 
 #include "kv_rope.cuh"
 
@@ -82,13 +86,26 @@ __device__ __forceinline__ float penalise(float x, float n, float rep, float fre
   return __fsub_rn(y, __fadd_rn(__fmul_rn(freq, n), pres));
 }
 
+// CTAs an SM: six (40 registers) hide the latency of a CTA's own phases; not where four chunks a
+// thread need the registers, nor for one row of one chunk (50258 bf16 logits: 3.1 us at four CTAs
+// an SM, 3.4 at six).
+constexpr int logit_ctas(int dtype, int u, int r) { return r == 1 && (u == 1 || dtype == 2) ? 4 : 6; }
+
 template <int kDtype, int kU, int kR>
-__global__ void __launch_bounds__(kLogitThreads, 4) logits_kernel(const LogitParams p) {
+__global__ void __launch_bounds__(kLogitThreads, logit_ctas(kDtype, kU, kR))
+    logits_kernel(const LogitParams p) {
   using T = LogitTile<kDtype, kU>;
   constexpr int kE = T::kE;
+  // Listed tokens are penalised as they stream by: single fp32 rows, whose chunks are four tokens
+  // (96 rows of 128001, histories to 16384: 44 us against 50 by the list; 256 bf16 rows of 32000,
+  // eight tokens a chunk, 16.8 against 14.6).
+  constexpr bool kInline = kR == 1 && kU > 1 && kDtype == 2;
+  // The history comes before the loads of the logits, so that its counting has their registers;
+  // behind them where a CTA has one chunk a thread and nothing else hides its latency.
+  constexpr bool kFirst = kR > 1 || kU > 1;
   constexpr uint32_t kAll = (1u << kE) - 1u;
   __shared__ uint32_t lsm[T::kWords];
-  __shared__ uint16_t list[T::kSpan];  // the slice's tokens that the history holds
+  __shared__ uint16_t list[kInline ? 1 : T::kSpan];  // the slice's tokens that the history holds
   __shared__ int n_list;
   uint32_t* const count = lsm;
   uint32_t* const seen = lsm + T::kSeen;
@@ -113,24 +130,40 @@ __global__ void __launch_bounds__(kLogitThreads, 4) logits_kernel(const LogitPar
     if (threadIdx.x == 0) n_list = 0;
     __syncthreads();
     const long long h0 = b * p.h_sb;
-    auto add = [&](long long v) {
-      const long long x = v - base;
-      if (v >= 0 && v < p.V && x >= 0 && x < T::kSpan && atomicAdd(&count[x], 1u) == 0) {
-        atomicOr(&seen[x >> 5], 1u << (x & 31));
-        list[atomicAdd(&n_list, 1)] = static_cast<uint16_t>(x);
+    // tokens [lo, lo + n_in) are counted here: one unsigned comparison a token
+    const int lo = max(base, 0), off = lo - base;
+    const uint32_t n_in = max(min(base + T::kSpan, p.V) - lo, 0);
+    auto add = [&](auto d) {
+      if (d < n_in) {
+        const uint32_t x = static_cast<uint32_t>(d) + off;
+        if (atomicAdd(&count[x], 1u) == 0) {
+          atomicOr(&seen[x >> 5], 1u << (x & 31));
+          if constexpr (!kInline) list[atomicAdd(&n_list, 1)] = static_cast<uint16_t>(x);
+        }
       }
     };
-    auto scan = [&](const auto* h) {  // 4 loads of a thread in flight
-      for (int i = threadIdx.x; i < n_hist; i += 4 * kLogitThreads) {
-        long long v[4];
+    auto scan = [&](const auto* h) {  // unsigned: a token below lo is far above lo + n_in, as ~0 is
+      using U = std::remove_cv_t<std::remove_reference_t<decltype(*h)>>;
+      const U low = static_cast<U>(lo);
+      U v[4];  // 4 loads of a thread in flight
+      int i = threadIdx.x;
+      if constexpr (kFirst) {
+        for (; i + 3 * kLogitThreads < n_hist; i += 4 * kLogitThreads) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = i + j * kLogitThreads < n_hist ? h[i + j * kLogitThreads] : -1;
+          for (int j = 0; j < 4; ++j) v[j] = h[i + j * kLogitThreads];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) add(v[j]);
+          for (int j = 0; j < 4; ++j) add(v[j] - low);
+        }
+      }
+      for (; i < n_hist; i += 4 * kLogitThreads) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = i + j * kLogitThreads < n_hist ? h[i + j * kLogitThreads] : ~U(0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) add(v[j] - low);
       }
     };
-    if (p.hist32) scan(reinterpret_cast<const int*>(p.history) + h0);
-    else scan(reinterpret_cast<const long long*>(p.history) + h0);
+    if (p.hist32) scan(reinterpret_cast<const uint32_t*>(p.history) + h0);
+    else scan(reinterpret_cast<const unsigned long long*>(p.history) + h0);
     __syncthreads();
   };
   // the mask's bits of the tokens [v0, v0 + kE)
@@ -151,6 +184,7 @@ __global__ void __launch_bounds__(kLogitThreads, 4) logits_kernel(const LogitPar
     }
   };
 
+  if (kFirst && n_hist > 0) count_history();
   // rows of one alignment: s0 + c, s0 + c + period, ...
   const int step = static_cast<int>(p.l_ss & (kE - 1));
   const int period = step == 0 ? 1 : kE / (step & -step);
@@ -213,11 +247,11 @@ __global__ void __launch_bounds__(kLogitThreads, 4) logits_kernel(const LogitPar
             }
           }
         }
-        if (!counted) {
+        if (!kFirst && !counted) {
           count_history();
           counted = true;
         }
-        if (bias != nullptr && n_hist > 0) {  // listed tokens stay as they are for now
+        if (!kInline && bias != nullptr && n_hist > 0) {  // listed tokens stay as they are for now
 #pragma unroll
           for (int u = 0; u < kU; ++u) {
             if (ok_all[u] == 0) continue;
@@ -237,14 +271,23 @@ __global__ void __launch_bounds__(kLogitThreads, 4) logits_kernel(const LogitPar
         for (int u = 0; u < kU; ++u) {
           if (v0[u] < 0 || v0[u] + kE > p.V) continue;  // an end of the row, below, or past it
           uint32_t w[4] = {raw[r][u].x, raw[r][u].y, raw[r][u].z, raw[r][u].w};
-          if (bias != nullptr) {
+          uint32_t hit = 0;  // one row: what the history holds of the chunk
+          if (kInline && n_hist > 0) {
+            const int x0 = v0[u] - base;
+            hit = __funnelshift_r(seen[x0 >> 5], seen[(x0 >> 5) + 1], x0 & 31) & ok[r][u];
+          }
+          if (bias != nullptr || hit != 0) {
+            auto value = [&](float x, int e) {
+              if (kInline && (hit >> e & 1u)) x = penalise(x, static_cast<float>(count[v0[u] - base + e]), rep, freq, pres);
+              return bias != nullptr ? __fadd_rn(x, bv[u][e]) : x;
+            };
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               if constexpr (kDtype == 2) {
-                w[j] = __float_as_uint(__fadd_rn(__uint_as_float(w[j]), bv[u][j]));
+                w[j] = __float_as_uint(value(__uint_as_float(w[j]), j));
               } else {
                 const float2 f = unpack2<kDtype == 0>(w[j]);
-                w[j] = pack2<kDtype == 0>(__fadd_rn(f.x, bv[u][2 * j]), __fadd_rn(f.y, bv[u][2 * j + 1]));
+                w[j] = pack2<kDtype == 0>(value(f.x, 2 * j), value(f.y, 2 * j + 1));
               }
             }
           }
@@ -288,11 +331,13 @@ __global__ void __launch_bounds__(kLogitThreads, 4) logits_kernel(const LogitPar
     float y = -INFINITY;
     if (m == nullptr || (m[v >> 5] >> (v & 31) & 1u)) {
       y = load_logit<kDtype>(in, v);
-      if (bias != nullptr && !(n_hist > 0 && count[v - base] != 0)) y = __fadd_rn(y, bias[v]);
+      const uint32_t n = n_hist > 0 ? count[v - base] : 0;
+      if (kInline && n != 0) y = penalise(y, static_cast<float>(n), rep, freq, pres);
+      if (bias != nullptr && (kInline || n == 0)) y = __fadd_rn(y, bias[v]);
     }
     store_logit<kDtype>(out0 + s * p.o_ss * T::kBytes, v, y);
   }
-  if (n_hist == 0) return;
+  if (kInline || n_hist == 0) return;
   // ---- the listed tokens ----
   __syncthreads();  // the rows are in `out`
   if constexpr (kR == 1) {

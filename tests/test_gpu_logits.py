@@ -113,6 +113,30 @@ def test_in_place_views_and_alignments():
         assert (wide[..., :off] == 5).all() and (wide[:, :, off + 2999:] == 5).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("B", [3, 700])
+def test_single_rows_in_views(B, dtype):
+    """One row a sequence, of rows at odd offsets, in place and into other strides; what the mask
+    forbids may be NaN and the history's tokens may lie at the rows' ends."""
+    V = 2600
+    d = make(7, B, 1, V, dtype, 80, "sequence", "row")
+    d["history"][:, :3] = torch.tensor([0, V - 1, 5], dtype=d["history"].dtype)
+    want = call(d)
+    check(d, want)
+    for off in (1, 2, 7):
+        wide = torch.full((B, 2, 2651), math.nan, dtype=dtype, device="cuda")
+        view = wide[:, 1:, off:off + V]
+        view.copy_(d["logits"].masked_fill(~d["allowed"], math.nan).cuda())
+        out = torch.full((B, 2613), 6.0, dtype=dtype, device="cuda")
+        got = call(d, logits=view, out=out[:, None, 3:3 + V])
+        assert torch.equal(got, want)
+        assert (out[:, :3] == 6).all() and (out[:, 3 + V:] == 6).all()
+        call(d, logits=view, out=view)
+        assert torch.equal(view, want) and wide[:, 0].isnan().all()
+        assert wide[..., :off].isnan().all() and wide[..., off + V:].isnan().all()
+    assert_device_ok()
+
+
 def test_infinities_nan_and_empty_masks():
     """NaN and infinities where the mask forbids do not matter; a row with nothing allowed is -inf
     throughout; -inf logits stay -inf through penalties."""
