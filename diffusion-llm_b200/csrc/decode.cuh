@@ -54,13 +54,15 @@ __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t& r0, uint32_t& r
                                         uint32_t& r2, uint32_t& r3) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
-               : "r"(addr));
+               : "r"(addr)
+               : "memory");
 }
 __device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t& r0, uint32_t& r1,
                                           uint32_t& r2, uint32_t& r3) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
-               : "r"(addr));
+               : "r"(addr)
+               : "memory");
 }
 template <bool kBF16>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
@@ -111,16 +113,20 @@ __device__ __forceinline__ int dec_split_entries(const DecParams& p, int bh, int
 
 // One 64-key K/V tile for the calling consumer warp (`warp` 0-3 takes keys [16 warp,
 // 16 warp + 16)): Q K^T and P V with mma.sync m16n8k16 and the online softmax of its rows
-// in registers. sk / sv: the tile's swizzled K and V in shared memory; the warp arrives on
-// `empty_bar` once its fragments are in registers. Keys at or past full_all are masked per
-// row against row_hi (the block-causal rule).
-template <int kMB, bool kBF16>
+// in registers. sk / sv: the tile's swizzled K and V in shared memory. Keys at or past
+// full_all are masked per row against row_hi (the block-causal rule). With kVEnd, V rows at or
+// past key v_end count as zero whatever they hold. The warp arrives on `empty_bar` once the
+// products have consumed its fragments: right after the ldmatrix loads is too early, with 32
+// rows the loads of V were seen behind the arrival, and a refill from L2 overwrote rows that
+// were still to be read (a few rows in 1 of 25 calls of the paged kernel).
+template <int kMB, bool kBF16, bool kVEnd = false>
 __device__ __forceinline__ void dec_tile_step(uint32_t sk, uint32_t sv, uint64_t* empty_bar,
                                               int warp, int lane, int key, int full_all,
                                               const int (&row_hi)[kMB][2],
                                               const uint32_t (&qa)[kMB][4][4],
                                               float (&acc)[kMB][8][4], float (&m_run)[kMB][2],
-                                              float (&l_run)[kMB][2], float scale_log2) {
+                                              float (&l_run)[kMB][2], float scale_log2,
+                                              int v_end = 0) {
   const int tq = lane & 3;
   // K fragments for this warp's 16 keys: 2 n-tiles x 4 k-steps
   uint32_t kb[4][4];
@@ -141,11 +147,19 @@ __device__ __forceinline__ void dec_tile_step(uint32_t sk, uint32_t sv, uint64_t
     ldsm_x4_t(sv + sw128_offset(vrow, chunk), vb[2 * dp][0], vb[2 * dp][1],
               vb[2 * dp + 1][0], vb[2 * dp + 1][1]);
   }
-  __syncwarp();
-  if (lane == 0) mbar_arrive(empty_bar);
 
   const int key0 = key + warp * 16;  // first key of this warp's slice
   const bool partial = key0 + 16 > full_all;
+  if (kVEnd && key0 + 16 > v_end) {
+    // zero the rows past v_end in V's fragments (a register holds keys 2tq, 2tq + 1 of 8)
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int c = key0 + half * 8 + 2 * tq;
+      const uint32_t keep = (c < v_end ? 0xFFFFu : 0u) | (c + 1 < v_end ? 0xFFFF0000u : 0u);
+#pragma unroll
+      for (int nt = 0; nt < 8; ++nt) vb[nt][half] &= keep;
+    }
+  }
 #pragma unroll
   for (int mb = 0; mb < kMB; ++mb) {
     float s[2][4];
@@ -200,6 +214,8 @@ __device__ __forceinline__ void dec_tile_step(uint32_t sk, uint32_t sv, uint64_t
 #pragma unroll
     for (int nt = 0; nt < 8; ++nt) mma16816<kBF16>(acc[mb][nt], pa, vb[nt][0], vb[nt][1]);
   }
+  __syncwarp();
+  if (lane == 0) mbar_arrive(empty_bar);
 }
 
 // ---- thread-block clusters (the split merge of a small decode) ----

@@ -172,93 +172,11 @@ __global__ void __launch_bounds__(kPgThreads, 2)
       const int st = J % S::kStages;
       ok = mbar_wait_warp(&full[st], (J / S::kStages) & 1);
       if (!ok) break;
-      const uint32_t sk = sbase + S::kRing + st * 2 * kPgTile, sv = sk + kPgTile;
-      uint32_t kb[4][4], vb[8][2];
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        const int mi = lane >> 3;
-        ldsm_x4(sk + sw128_offset(warp * 16 + (mi >> 1) * 8 + (lane & 7), ks * 2 + (mi & 1)),
-                kb[ks][0], kb[ks][1], kb[ks][2], kb[ks][3]);
-      }
-#pragma unroll
-      for (int dp = 0; dp < 4; ++dp) {
-        const int mi = lane >> 3;
-        ldsm_x4_t(sv + sw128_offset(warp * 16 + (mi & 1) * 8 + (lane & 7), dp * 2 + (mi >> 1)),
-                  vb[2 * dp][0], vb[2 * dp][1], vb[2 * dp + 1][0], vb[2 * dp + 1][1]);
-      }
-
-      const int key0 = t * kPgBN + warp * 16;  // first key of this warp's slice
-      const bool partial = key0 + 16 > full_all;
-      if (key0 + 16 > it.hi) {
-        // Rows of the page past the visible keys hold anything, NaN included, and P = 0 does not
-        // cancel that: zero them in V's fragments (a register holds keys 2tq, 2tq + 1 of 8).
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int c = key0 + half * 8 + 2 * tq;
-          const uint32_t keep = (c < it.hi ? 0xFFFFu : 0u) | (c + 1 < it.hi ? 0xFFFF0000u : 0u);
-#pragma unroll
-          for (int nt = 0; nt < 8; ++nt) vb[nt][half] &= keep;
-        }
-      }
-#pragma unroll
-      for (int mb = 0; mb < kMB; ++mb) {
-        float s[2][4];
-#pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[nt][i] = 0.f;
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-          mma16816<kBF16>(s[0], qa[mb][ks], kb[ks][0], kb[ks][1]);
-          mma16816<kBF16>(s[1], qa[mb][ks], kb[ks][2], kb[ks][3]);
-        }
-        if (partial) {
-#pragma unroll
-          for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (key0 + nt * 8 + 2 * tq + (i & 1) >= row_hi[mb][i >> 1]) s[nt][i] = -INFINITY;
-        }
-#pragma unroll
-        for (int hr = 0; hr < 2; ++hr) {
-          float mx = fmaxf(fmaxf(s[0][2 * hr], s[0][2 * hr + 1]),
-                           fmaxf(s[1][2 * hr], s[1][2 * hr + 1]));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          const float m_new = fmaxf(m_run[mb][hr], mx * p.scale_log2);
-          const float m_use = m_new == -INFINITY ? 0.f : m_new;
-          const float alpha = ex2(m_run[mb][hr] - m_use);
-          m_run[mb][hr] = m_new;
-          float rs = 0.f;
-#pragma unroll
-          for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const float e = ex2(fmaf(s[nt][2 * hr + i], p.scale_log2, -m_use));
-              s[nt][2 * hr + i] = e;
-              rs += e;
-            }
-          l_run[mb][hr] = l_run[mb][hr] * alpha + rs;
-#pragma unroll
-          for (int nt = 0; nt < 8; ++nt) {
-            acc[mb][nt][2 * hr] *= alpha;
-            acc[mb][nt][2 * hr + 1] *= alpha;
-          }
-        }
-        uint32_t pa[4];
-        pa[0] = pack2<kBF16>(s[0][0], s[0][1]);
-        pa[1] = pack2<kBF16>(s[0][2], s[0][3]);
-        pa[2] = pack2<kBF16>(s[1][0], s[1][1]);
-        pa[3] = pack2<kBF16>(s[1][2], s[1][3]);
-#pragma unroll
-        for (int nt = 0; nt < 8; ++nt) mma16816<kBF16>(acc[mb][nt], pa, vb[nt][0], vb[nt][1]);
-      }
-      // The slot is given back once the products have consumed the fragments. Giving it back
-      // right after the ldmatrix loads was measured to be too early: with 32 rows the loads of V
-      // ended up behind the arrival, and a refill from L2 overwrote rows that were still to be
-      // read (a few rows in 1 of 25 calls).
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[st]);
+      const uint32_t sk = sbase + S::kRing + st * 2 * kPgTile;
+      // Rows of the page past the visible keys hold anything, NaN included, and P = 0 does not
+      // cancel that: V's count as zero.
+      dec_tile_step<kMB, kBF16, true>(sk, sk + kPgTile, &empty[st], warp, lane, t * kPgBN, full_all,
+                                      row_hi, qa, acc, m_run, l_run, p.scale_log2, it.hi);
     }
 
     // ---- merge the four warps' states (each row's sum is still spread over its quad) ----
