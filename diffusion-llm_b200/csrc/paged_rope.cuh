@@ -59,7 +59,7 @@ __global__ void __launch_bounds__(256) qkv_rope_paged_kernel(const PagedRopePara
     int b = b0;
     while (b < p.B && p.cu_q[b + 1] <= t) ++b;
     int pos = -1, page = 0, row = 0;
-    if (b < p.B) {  // tokens past cu_q[B] belong to no sequence
+    if (b < p.B && t >= p.cu_q[b]) {  // tokens before cu_q[0] or past cu_q[B] are in no sequence
       const long long at = static_cast<long long>(p.kv_lens[b]) - p.cu_q[b + 1] + t;
       const long long pg = at / p.page_size;
       bool ok = at >= 0 && at < p.max_pos && pg < p.max_pages;

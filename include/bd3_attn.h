@@ -286,8 +286,9 @@ BD3_API int bd3_subs_sample_dev(const void* logits, const int64_t* logit_strides
  *     are not read.
  *   cu_q: device int32 (B + 1), kv_lens: device int32 (B). The new tokens of all sequences are
  *     packed: sequence b has rows [cu_q[b], cu_q[b+1]) and they are the last of its kv_lens[b]
- *     positions (the new tokens counted). A sequence may have no new tokens. Rows at or past
- *     cu_q[B] belong to no sequence and are left alone.
+ *     positions (the new tokens counted). A sequence may have no new tokens. Rows before
+ *     cu_q[0] (a sub-batch passes its part of the offsets) and rows at or past cu_q[B] belong to
+ *     no sequence and are left alone.
  *
  * bd3_paged_attn: block-causal attention of the new tokens: a token at position p sees the
  * positions [0, min((p / block_size + 1) * block_size, kv_len)) of its sequence (the rule of

@@ -449,3 +449,67 @@ def test_write_then_attend():
     assert_device_ok()
     assert torch.equal(whole["k_pages"].nan_to_num(9), parts["k_pages"].nan_to_num(9))
     assert (o.float() - o2.float()).abs().max() <= 2 * 2.0 ** -8 * 4.5  # two roundings of |O| < 4.5 each
+
+# ---- packed rows that belong to no sequence ----------------------------------------------------
+
+@pytest.mark.parametrize("first", [1, 3, 40, 700])
+def test_rope_write_leaves_the_rows_before_the_first_sequence_alone(first):
+    """A sub-batch over the whole packed projection: rows before cu_q[0] are in no sequence, though
+    the first sequence has earlier positions that they would count back to."""
+    Hq, Hkv = 4, 2
+    d, dev = rope_case(12, [(5, 800), (0, 30), (2, 3)], Hq, Hkv, 64, 16, torch.bfloat16)
+    g = torch.Generator().manual_seed(13)
+    before = torch.randn(first, 8 * 64, generator=g).bfloat16()
+    d["qkv"] = torch.cat([before, d["qkv"]])
+    d["cu_q"] = d["cu_q"] + first
+    dev["qkv"], dev["cu_q"] = d["qkv"].cuda(), d["cu_q"].cuda()
+    out = torch.full((first + 7, Hq, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+    q = write(dev, Hq, Hkv, q_out=out)
+    assert_device_ok()
+    assert (q[:first] == 7).all()
+    rq, rk, rv = op.rope_write(d["qkv"], Hq, Hkv, d["cos"], d["sin"], d["k_pages"], d["v_pages"],
+                               d["page_table"], d["kv_lens"], d["cu_q"])
+    assert torch.equal(dev["v_pages"].cpu().double(), rv)
+    for got, ref in ((q[first:], rq[first:]), (dev["k_pages"], rk)):
+        assert ((got.cpu().double() - ref).abs() <= 1.01 * 2.0 ** -8 * ref.abs() + 2e-6).all()
+    touched = (rk != d["k_pages"].double()).any(-1).any(1)  # (page, row)
+    assert torch.equal(dev["k_pages"].cpu().transpose(1, 2)[~touched], d["k_pages"].transpose(1, 2)[~touched])
+
+
+def test_offsets_that_run_back_reach_no_other_row():
+    """Offsets that run back are outside the contract: the write touches no row but those that the
+    offsets name, the attention reports them (status bit 2)."""
+    from bd3attn import ops
+    d, dev = rope_case(14, [(4, 300), (4, 90)], 4, 2, 64, 16, torch.bfloat16)
+    dev["cu_q"] = torch.tensor([6, 8, 4], dtype=torch.int32, device="cuda")
+    q = write(dev, 4, 2)
+    assert_device_ok()
+    k = d["k_pages"].clone()
+    page = d["page_table"]
+    touched = torch.zeros(k.shape[0], 16, dtype=torch.bool)
+    for pos in (298, 299):  # rows 6 and 7 are the first sequence's last positions
+        touched[page[0, pos // 16].long(), pos % 16] = True
+    assert torch.equal(dev["k_pages"].cpu().transpose(1, 2)[~touched], k.transpose(1, 2)[~touched])
+    ops.paged_attn_raw(q, dev["k_pages"], dev["v_pages"], dev["page_table"], dev["kv_lens"], dev["cu_q"], 2, 16)
+    torch.cuda.synchronize()
+    assert ops.device_status() == 2
+
+
+@pytest.mark.parametrize("rows", [16, 160])
+def test_attention_of_a_sub_batch(rows):
+    """cu_q[k:], kv_lens[k:] and page_table[k:] over the whole packed q: the rows of the sequences
+    left out, before cu_q[0] and past cu_q[B], belong to no sequence."""
+    lens = [(rows, 700), (rows, 90 + rows), (7, 333), (rows, rows)]
+    d, dev = make(61, lens, 4, 2, 16, torch.bfloat16)
+    for x in (d, dev):
+        x.update(cu_q=x["cu_q"][1:4], kv_lens=x["kv_lens"][1:3], page_table=x["page_table"][1:3])
+    d["kv_lens"], dev["kv_lens"] = d["kv_lens"].clone(), dev["kv_lens"].clone()
+    dev["cu_q"] = dev["cu_q"].clone()
+    o, lse = run(dev, lens, 16, return_lse=True)
+    assert_device_ok()
+    part = slice(rows, 2 * rows + 7)
+    ref, ref_lse, mag = op.paged_attention(d["q"], d["k_pages"], d["v_pages"], d["page_table"], d["kv_lens"],
+                                           d["cu_q"], 16)
+    err = (o.cpu().double() - ref).abs()[part]
+    assert (err <= (1.1 * 2.0 ** -8 * (ref.abs() + mag) + 1e-6)[part]).all()
+    assert ((lse.cpu().double() - ref_lse).abs()[part] <= LSE_TOL).all()
