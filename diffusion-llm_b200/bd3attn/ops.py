@@ -434,10 +434,12 @@ def paged_attn_raw(q, k_pages, v_pages, page_table, kv_lens, cu_q, max_q_len: in
     q: (tokens, q heads, 64) bf16/f16, sequence b's rows [cu_q[b], cu_q[b+1]); k_pages, v_pages:
     (pages, kv heads, page size, 64) in q's dtype, any strides, page size a multiple of 8;
     page_table: (B, pages per sequence) int32; kv_lens: (B,) int32 positions of each sequence,
-    the new tokens (its last ones) included; cu_q: (B + 1,) int32; max_q_len: the most new
-    tokens of a sequence. Tensors of lengths stay on the device: a captured CUDA graph serves
-    other lengths and tables. workspace: paged_workspace(), kept by the caller (None: a new
-    zeroed one). Returns O (tokens, q heads, 64), with the LSE (tokens, q heads) if asked.
+    the new tokens (its last ones) included; cu_q: (B + 1,) int32, rows before its first and past
+    its last entry are in no sequence and their output is undefined; max_q_len: the most new
+    tokens of a sequence (one with more is cut and sets device status bit 2). Tensors of lengths
+    stay on the device: a captured CUDA graph serves other lengths and tables. workspace:
+    paged_workspace(), kept by the caller (None: a new zeroed one). Returns O (tokens, q heads,
+    64), with the LSE (tokens, q heads) if asked.
     Forward only, as the other decode functions.
     """
     _check_cuda(q)
@@ -449,6 +451,9 @@ def paged_attn_raw(q, k_pages, v_pages, page_table, kv_lens, cu_q, max_q_len: in
     if q.dim() != 3:
         raise AssertionError("q must be (tokens, q heads, head_dim)")
     T, Hq, D = q.shape
+    max_q_len = int(max_q_len)
+    if max_q_len < 1 and T > 0:
+        raise AssertionError("max_q_len must be >= 1 where there are tokens")
     n_pages, Hkv, page_size = k_pages.shape[:3] if k_pages.dim() == 4 else (0, 0, 0)
     B, width, ks, vs = _check_pages(k_pages, v_pages, page_table, kv_lens, cu_q, q.dtype, Hkv, D)
     qs = q.stride()
@@ -469,7 +474,7 @@ def paged_attn_raw(q, k_pages, v_pages, page_table, kv_lens, cu_q, max_q_len: in
     rc = LIB.bd3_paged_attn(
         q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), o.data_ptr(),
         lse.data_ptr() if return_lse else None, page_table.data_ptr(), kv_lens.data_ptr(),
-        cu_q.data_ptr(), B, T, int(max_q_len), Hq, Hkv, D, n_pages, page_size, width,
+        cu_q.data_ptr(), B, T, max_q_len, Hq, Hkv, D, n_pages, page_size, width,
         _I64x11(qs[0], qs[1], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], Hq * D, D,
                 page_table.stride(0)),
         int(block_size), D ** -0.5 if scale is None else float(scale), code, out_code,

@@ -296,7 +296,8 @@ BD3_API int bd3_subs_sample_dev(const void* logits, const int64_t* logit_strides
  * sees none (kv_len below the new tokens' count) gets O = 0 and LSE = -inf. Query heads h share
  * KV head h / (Hq / Hkv). What lies in a page past kv_len is never used (NaN included).
  *   q, o: (total_q, Hq, 64), o in dtype or fp32; lse: optional (total_q, Hq) fp32 contiguous.
- *   max_q: the most new tokens of a sequence (host). page_size % 8 == 0.
+ *   max_q: the most new tokens of a sequence (host); 0 says that there are none, and nothing is
+ *     launched or written. page_size % 8 == 0.
  *   strides[11] = q (token, head), k_pages, v_pages (page, head, row), o (token, head),
  *     page_table (sequence), in elements. scale: of the scores, usually 1 / sqrt(D).
  *   workspace: bd3_paged_workspace_size() bytes on the current device, zeroed once by the

@@ -513,3 +513,19 @@ def test_attention_of_a_sub_batch(rows):
     err = (o.cpu().double() - ref).abs()[part]
     assert (err <= (1.1 * 2.0 ** -8 * (ref.abs() + mag) + 1e-6)[part]).all()
     assert ((lse.cpu().double() - ref_lse).abs()[part] <= LSE_TOL).all()
+
+
+def test_no_length_for_the_tokens_is_refused():
+    """max_q_len 0 (or less) beside tokens would leave the output as it was allocated."""
+    from bd3attn import ops
+    lens = [(16, 100), (3, 40)]
+    _, dev = make(62, lens, 4, 2, 16, torch.bfloat16)
+    args = [dev[k] for k in ("q", "k_pages", "v_pages", "page_table", "kv_lens", "cu_q")]
+    for n in (0, -1):
+        with pytest.raises(AssertionError, match="max_q_len"):
+            ops.paged_attn_raw(*args, n, 16)
+        with pytest.raises(AssertionError, match="max_q_len"):
+            ops.paged_attn_raw(*args, n, 16, return_lse=True, workspace=ops.paged_workspace("cuda"))
+    o, lse = ops.paged_attn_raw(args[0][:0], *args[1:5], torch.zeros_like(dev["cu_q"]), 0, 16, return_lse=True)
+    assert o.shape == (0, 4, 64) and lse.shape == (0, 4)  # no tokens: nothing to do
+    assert_device_ok()
