@@ -60,6 +60,7 @@ class PagedKVCache:
         self._len: dict[int, int] = {}           # sequence -> committed positions
         self._next = 0
         self._new: dict[int, int] = {}           # the current begin()
+        self._open = False                       # between begin() and commit()
         self.max_new = self.tokens = 0
         self._workspace = None
 
@@ -109,7 +110,7 @@ class PagedKVCache:
             rows.append(pages + [0] * (width - len(pages)))
             cu.append(cu[-1] + n)
             lens.append(total)
-        self._new = dict(new)
+        self._new, self._open = dict(new), True
         self.max_new, self.tokens = max(new.values(), default=0), cu[-1]
         # sequences past the last one have no tokens and no positions
         spare = self.max_seqs - len(new)
@@ -124,13 +125,21 @@ class PagedKVCache:
         """The new positions of the last begin() stay."""
         for seq, n in self._new.items():
             self._len[seq] += n
-        self._new, self.max_new, self.tokens = {}, 0, 0
+        self._new, self.max_new, self.tokens, self._open = {}, 0, 0, False
+
+    def _check_step(self, rows: int) -> None:
+        """The device holds the last begin()'s lengths and table: of use until its commit() only."""
+        if not self._open:
+            raise RuntimeError("rope_qkv and attend belong between begin() and commit()")
+        if rows < self.tokens:
+            raise AssertionError(f"{rows} rows for the step's {self.tokens} new tokens")
 
     def rope_qkv(self, layer_idx: int, qkv: torch.Tensor, n_heads: int, cos_table: torch.Tensor,
                  sin_table: torch.Tensor, q_out: torch.Tensor | None = None) -> torch.Tensor:
         """Rotated queries (tokens, n_heads, head_dim) of the layer's packed QKV projection
         (tokens, (n_heads + 2 * n_kv_heads) * head_dim); its rotated keys and its values go
-        into the layer's pages."""
+        into the layer's pages. RuntimeError outside a step (begin() to commit())."""
+        self._check_step(qkv.shape[0])
         return ops.qkv_rope_paged_raw(qkv, n_heads, self.n_kv_heads, cos_table, sin_table,
                                       self.k[layer_idx], self.v[layer_idx], self.page_table,
                                       self.kv_lens, self.cu_q, q_out=q_out)
@@ -139,9 +148,10 @@ class PagedKVCache:
                return_lse: bool = False):
         """Block-causal attention (tokens, n_heads, head_dim) of the new tokens over their
         sequences' committed and new positions. The cache's calls share its workspace: they
-        must be ordered, as on one stream."""
+        must be ordered, as on one stream. RuntimeError outside a step (begin() to commit())."""
+        self._check_step(q.shape[0])
         if self._workspace is None:
             self._workspace = ops.paged_workspace(q.device)
         return ops.paged_attn_raw(q, self.k[layer_idx], self.v[layer_idx], self.page_table,
-                                  self.kv_lens, self.cu_q, self.max_new, block_size,
+                                  self.kv_lens, self.cu_q, max(self.max_new, 1), block_size,
                                   return_lse=return_lse, workspace=self._workspace)

@@ -143,3 +143,22 @@ def test_a_captured_step_serves_growing_sequences(model):
             ref = full_logits(model, s)
             err = (torch.cat([x[i] for x in got]).float() - ref).abs().max().item()
             assert err <= 0.03 * max(1.0, ref.abs().max().item()), (i, err)
+
+
+def test_padding_rows_and_a_step_without_new_tokens():
+    """More rows than the step has tokens: the rest is in no sequence; a step of no tokens at all
+    writes nothing and reports nothing."""
+    from bd3attn.paged_cache import PagedKVCache
+    cache = PagedKVCache(1, 2, 8, 2, 64, page_size=16)
+    a = cache.add()
+    tab = torch.ones(64, 32, device="cuda")
+    qkv = torch.randn(8, 8 * 64, device="cuda").bfloat16()
+    for n in (5, 0):
+        cache.begin({a: n})
+        before = cache.v[0].clone()
+        q = cache.rope_qkv(0, qkv, 4, tab, tab)
+        o, lse = cache.attend(0, q, 1, return_lse=True)
+        assert o.shape == (8, 4, 64) and torch.isfinite(o[:n]).all() and torch.isfinite(lse[:n]).all()
+        assert int((cache.v[0] != before).flatten(1).any(1).sum()) == (n > 0)
+        cache.commit()
+    assert_device_ok()

@@ -68,3 +68,31 @@ def test_refusals_change_nothing():
     for kw in (dict(page_size=12), dict(num_pages=0), dict(max_len=0)):
         with pytest.raises(ValueError):
             cache(**kw)
+
+
+def test_no_write_or_attention_outside_a_step():
+    """Before the first begin() and after commit() nothing is new: the device still holds the last
+    step's lengths, so both calls are refused; so are fewer rows than the step has."""
+    c = cache()
+    a = c.add()
+    qkv, q, tab = torch.zeros(5, 12 * 64), torch.zeros(5, 6, 64), torch.ones(64, 32)
+
+    def refused(kind, match, rows=5):
+        with pytest.raises(kind, match=match):
+            c.rope_qkv(0, qkv[:rows], 6, tab, tab)
+        with pytest.raises(kind, match=match):
+            c.attend(0, q[:rows], 1)
+
+    refused(RuntimeError, "begin")
+    c.begin({a: 5})
+    refused(AssertionError, "5 new tokens", 4)
+    c.commit()
+    refused(RuntimeError, "begin")
+    assert c.length(a) == 5
+    with pytest.raises(RuntimeError, match="max_len"):
+        c.begin({a: 60})
+    refused(RuntimeError, "begin")  # a refused begin() opens nothing
+    c.begin({a: 4})
+    with pytest.raises(RuntimeError, match="max_len"):
+        c.begin({a: 60})
+    refused(AssertionError, "4 new tokens", 3)  # and leaves an open step as it is
