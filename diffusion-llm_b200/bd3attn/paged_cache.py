@@ -73,11 +73,12 @@ class PagedKVCache:
         return seq
 
     def release(self, seq: int) -> None:
-        """End a sequence: its pages go back to the pool."""
+        """End a sequence: its pages go back to the pool. In the middle of a step the packed rows
+        stay as they are (the pages serve others from the next begin() on) and the other
+        sequences commit theirs."""
         self._free.extend(reversed(self._pages.pop(seq)))
         del self._len[seq]
-        if self._new.pop(seq, None) is not None:
-            self._new, self.max_new, self.tokens = {}, 0, 0
+        self._new.pop(seq, None)
 
     def length(self, seq: int) -> int:
         """Committed positions of a sequence."""

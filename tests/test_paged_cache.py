@@ -96,3 +96,27 @@ def test_no_write_or_attention_outside_a_step():
     with pytest.raises(RuntimeError, match="max_len"):
         c.begin({a: 60})
     refused(AssertionError, "4 new tokens", 3)  # and leaves an open step as it is
+
+
+def test_release_in_a_step_leaves_the_others_in_it():
+    """A sequence that ends in mid-step takes its pages and nothing else along: the packed rows stay
+    as they are and the others commit."""
+    c = cache()
+    a, b = c.add(), c.add()
+    c.begin({a: 17, b: 20})
+    c.release(a)
+    assert c.free_pages == 8 and (c.max_new, c.tokens) == (20, 37)
+    assert c.cu_q.tolist() == [0, 17, 37, 37]
+    with pytest.raises(AssertionError, match="37 new tokens"):
+        c.attend(0, torch.zeros(20, 6, 64), 1)
+    c.commit()
+    assert c.length(b) == 20
+    with pytest.raises(KeyError):
+        c.length(a)
+    c.begin({b: 3})
+    c.release(b)
+    assert c.free_pages == 10
+    c.commit()  # nothing is left in the step
+    d = c.add()
+    c.begin({d: 16})
+    assert c.kv_lens.tolist() == [16, 0, 0] and c.free_pages == 9
