@@ -62,7 +62,8 @@ class PagedKVCache:
         self._new: dict[int, int] = {}           # the current begin()
         self._open = False                       # between begin() and commit()
         self.max_new = self.tokens = 0
-        self._workspace = None
+        # of attend; made here, since a zeroing that a graph capture records runs only at its replays
+        self._workspace = ops.paged_workspace(self.page_table.device) if self.page_table.is_cuda else None
 
     def add(self) -> int:
         """A new, empty sequence; returns its handle."""
@@ -151,8 +152,6 @@ class PagedKVCache:
         sequences' committed and new positions. The cache's calls share its workspace: they
         must be ordered, as on one stream. RuntimeError outside a step (begin() to commit())."""
         self._check_step(q.shape[0])
-        if self._workspace is None:
-            self._workspace = ops.paged_workspace(q.device)
         return ops.paged_attn_raw(q, self.k[layer_idx], self.v[layer_idx], self.page_table,
                                   self.kv_lens, self.cu_q, max(self.max_new, 1), block_size,
                                   return_lse=return_lse, workspace=self._workspace)

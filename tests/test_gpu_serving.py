@@ -162,3 +162,37 @@ def test_padding_rows_and_a_step_without_new_tokens():
         assert int((cache.v[0] != before).flatten(1).any(1).sum()) == (n > 0)
         cache.commit()
     assert_device_ok()
+
+
+def test_a_step_captured_on_a_new_cache_leaves_eager_calls_right():
+    """The first attention of a cache may be the one that a graph captures: an eager call before
+    the first replay, the replay and a call after it all give the same bits."""
+    from bd3attn import ops
+    from bd3attn.paged_cache import PagedKVCache
+
+    def new():
+        cache = PagedKVCache(1, 2, 128, 1, 2048, page_size=16)
+        a = cache.add()
+        cache.begin({a: 1984})
+        cache.commit()
+        cache.begin({a: 16})
+        for x in (cache.k[0], cache.v[0]):
+            x.normal_(generator=torch.Generator("cuda").manual_seed(5))
+        return cache
+
+    q = torch.randn(16, 4, 64, device="cuda").bfloat16()
+    new().attend(0, -q, 16)  # the library's own first call
+    first, graph = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(first):  # an earlier graph of the same pool leaves its memory as it used it
+        junk = torch.full((1 << 28,), 0xA5, dtype=torch.uint8, device="cuda")
+    first.replay()
+    del junk
+    cache = new()
+    with torch.cuda.graph(graph, pool=first.pool()):
+        out = cache.attend(0, q, 16)
+    eager = cache.attend(0, q, 16).clone()
+    graph.replay()
+    after = cache.attend(0, q, 16)
+    ref = ops.paged_attn_raw(q, cache.k[0], cache.v[0], cache.page_table, cache.kv_lens, cache.cu_q, 16, 16)
+    assert_device_ok()
+    assert torch.equal(eager, ref) and torch.equal(out, ref) and torch.equal(after, ref)
