@@ -72,12 +72,23 @@ class PagedGeneration:
             allowed: torch.Tensor | None = None) -> list[torch.Tensor]:
         """Generate n_blocks[i] blocks after prompts[i] (int64 device tokens, whole blocks).
         allowed: packed words (pack_mask) of the tokens that may be generated, (words,) or one
-        row per sequence. Returns each sequence's generated tokens."""
+        row per sequence. Returns each sequence's generated tokens. Whatever ends the run, an error
+        among it, the cache has its sequences' pages back."""
         if any(len(p) % self.bs for p in prompts):
             raise ValueError("prompts must be whole blocks")
+        seqs: dict[int, int] = {}  # prompt -> its sequence while it has one
+        try:
+            for i in range(len(prompts)):
+                if n_blocks[i] > 0:
+                    seqs[i] = self.cache.add()
+            return self._generate(prompts, n_blocks, allowed, seqs)
+        finally:
+            for s in seqs.values():
+                self.cache.release(s)
+
+    def _generate(self, prompts, n_blocks, allowed, seqs) -> list[torch.Tensor]:
         dev, bs, mask = self.cos.device, self.bs, self.m.mask_index
-        seqs = [self.cache.add() for _ in prompts]
-        self.prefill({s: p for s, p in zip(seqs, prompts) if len(p)})
+        self.prefill({s: prompts[i] for i, s in seqs.items() if len(prompts[i])})
         buf = torch.zeros((len(prompts), self.max_len), dtype=torch.int64, device=dev)
         for i, p in enumerate(prompts):
             buf[i, :len(p)] = p
@@ -105,5 +116,5 @@ class PagedGeneration:
             for i in live:
                 done[i] += 1
                 if done[i] == n_blocks[i]:
-                    self.cache.release(seqs[i])
+                    self.cache.release(seqs.pop(i))
         return [buf[i, len(p):len(p) + done[i] * bs].clone() for i, p in enumerate(prompts)]

@@ -196,3 +196,42 @@ def test_a_step_captured_on_a_new_cache_leaves_eager_calls_right():
     ref = ops.paged_attn_raw(q, cache.k[0], cache.v[0], cache.page_table, cache.kv_lens, cache.cu_q, 16, 16)
     assert_device_ok()
     assert torch.equal(eager, ref) and torch.equal(out, ref) and torch.equal(after, ref)
+
+
+def test_every_way_out_of_a_run_returns_its_sequences(model):
+    """Sequences of no blocks, a request past max_len, a pool that runs out, more prompts than
+    sequences, a backbone that fails in mid-step: pages and places are back each time."""
+    from workloads.serving import PagedGeneration
+    g = torch.Generator().manual_seed(6)
+    gen = PagedGeneration(model, 3, 128, 20, page_size=16, steps=2, chunk=32)
+
+    def prompts(*lens):
+        return [torch.randint(0, V - 1, (n,), generator=g).cuda() for n in lens]
+
+    def free():
+        for s in [gen.cache.add() for _ in range(3)]:
+            gen.cache.release(s)
+        return gen.cache.free_pages == 20
+
+    assert [len(o) for o in gen.run(prompts(32, 16, 0), [0, 1, 0])] == [0, 16, 0]
+    assert free()
+    for lens, blocks in (((112, 16), [2, 1]), ((112, 112, 112), [1, 1, 1]), ((16,) * 4, [1] * 4), ((16, 16), [1])):
+        with pytest.raises((RuntimeError, IndexError)):
+            gen.run(prompts(*lens), blocks)
+        assert free(), (lens, blocks)
+    forward, calls = gen.forward, []
+
+    def failing(*a, **kw):
+        calls.append(1)
+        if len(calls) == 3:
+            raise ValueError("a step that fails")
+        return forward(*a, **kw)
+
+    gen.forward = failing
+    with pytest.raises(ValueError, match="a step that fails"):
+        gen.run(prompts(32, 16), [2, 2])
+    gen.forward = forward
+    assert free()
+    assert [len(o) for o in gen.run(prompts(96, 16, 0), [1, 2, 3])] == [16, 32, 48]
+    assert free()
+    assert_device_ok()
