@@ -47,7 +47,9 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None,
 
     With n the occurrences of token v among the first history_len[b] entries of history[b]:
     x = logits; if n > 0, x = (x / repetition if x > 0 else x * repetition) - (frequency * n +
-    presence); x += bias; x = -inf where the mask forbids v. fp32 arithmetic, rounded once.
+    presence); x += bias; x = -inf where the mask forbids v. fp32 arithmetic, rounded once. One
+    history serves the three penalties: where frequency and presence are to count the generated
+    tokens only (the repetition penalty the prompt's as well), call it once for each.
 
     logits: bf16, f16 or fp32; history: (batch, capacity) int64 or int32 tokens (ids outside the
     vocabulary, padding for one, are ignored) with history_len (batch,) int32; repetition (> 0),

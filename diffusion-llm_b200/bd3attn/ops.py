@@ -416,7 +416,8 @@ def _check_pages(k_pages, v_pages, page_table, kv_lens, cu_q, dtype, n_kv_heads,
 
 def paged_workspace(device=None) -> torch.Tensor:
     """A workspace for paged_attn_raw on `device` (bd3_paged_workspace_size bytes, zeroed). Keep
-    it and pass it to every call; calls that share one must be ordered (one stream)."""
+    it and pass it to every call; calls that share one must be ordered (one stream). Not to be
+    made under a graph capture: the zeroing would run at the graph's replays."""
     device = torch.device("cuda", torch.cuda.current_device()) if device is None \
         else torch.device(device)
     with torch.cuda.device(device):

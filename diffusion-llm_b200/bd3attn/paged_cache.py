@@ -19,7 +19,7 @@ writes them again (a denoising step that repeats the block with other tokens), a
 ``begin`` starts from the committed lengths. ``begin`` is the only place where the host tells
 the device anything (page table, lengths, offsets); the layers' calls read them there, so one
 step can be captured in a CUDA graph and replayed for as long as the numbers of new tokens stay
-the same.
+the same. Between ``commit`` and the next ``begin`` there is no step, and the layers' calls raise.
 """
 
 from __future__ import annotations
@@ -37,6 +37,7 @@ class PagedKVCache:
         num_pages: pages of the pool (each holds page_size positions of every layer).
         max_seqs: sequences at a time; max_len: positions of one sequence at most.
         page_size: positions per page, a multiple of 8.
+        dtype: bf16 or f16 (rope_qkv also takes fp32, attend does not).
     """
 
     def __init__(self, n_layers: int, n_kv_heads: int, num_pages: int, max_seqs: int, max_len: int,

@@ -1204,8 +1204,9 @@ constexpr int kPagedCtas = 2;  // CTAs an SM of paged_attn_kernel (paged_attn_tc
 constexpr int kPagedWorkers = bd3::kPtWorkers > kPagedCtas ? bd3::kPtWorkers : kPagedCtas;
 
 // Rows per sequence and KV head up to which paged_attn_kernel takes a call, paged_attn_tc_kernel
-// above it. At 32 rows, 12 heads: 64 sequences of 332 positions 38 us against 39, one of 132
-// 10.0 against 11.6, two of 65568 88 against 85; at 64 rows of those two 165 against 85.
+// above it. At 32 rows, 12 heads: 64 sequences of 332 positions 35 us against 39, one of 132
+// 9.7 against 11.4, two of 65568 90 against 86; at 64 rows, two of 65600 155 against 87, one of
+// 164 9.7 against 11.9.
 constexpr int64_t kPagedMaxRows = 32;
 
 // Counts (zero between calls), then the partials of the widest kernel's row tile.
@@ -1394,7 +1395,8 @@ int bd3_qkv_rope_paged(const void* qkv, int64_t qkv_stride, int64_t T, int64_t B
   p.page_size = static_cast<int>(page_size);
   p.max_pages = static_cast<int>(max_pages);
   // tokens per CTA: 4 (fewer searches for a token's sequence), fewer while SMs would idle (64
-  // tokens of 48 heads: 2.9 us at 1, 4.4 at 4; 5753 tokens: 21.0 at 1, 15.5 at 4, 19.4 at 16)
+  // tokens of 48 heads: 3.3 us at 1, 4.6 at 4; 5753 f16 tokens of 48 heads: 21.1 at 1, 16.6 at 4,
+  // 20.2 at 16)
   p.tpb = static_cast<int>(T / (2 * sms) < 1 ? 1 : T / (2 * sms) > 4 ? 4 : T / (2 * sms));
   auto kern = dtype == BD3_BF16  ? bd3::qkv_rope_paged_kernel<0>
               : dtype == BD3_F16 ? bd3::qkv_rope_paged_kernel<1>
@@ -1426,10 +1428,14 @@ int launch_logits_u(bd3::LogitParams& p, int64_t B, int sms, void* stream) {
                     "logits_kernel launch", p);
 }
 // Several rows: two of one alignment at a time (four leave five CTAs an SM: 32 x 8 rows of 50257
-// fp32 31 us against 28, 8 x 16 of 50258 bf16 16.5 against 14.2). One row: 4096 tokens a CTA where
-// that leaves four CTAs an SM (fewer CTAs scan the history: 96 fp32 rows of 128001 with 16384
-// tokens each 81 us against 93 at 2048, with 1024 each 40 against 38.5), else one chunk a thread
-// (one row of 50258 bf16: 2.3 us against 2.7).
+// fp32 31 us against 28, 8 x 16 of 50258 bf16 16.5 against 14.2). One row: one chunk a thread
+// (1024 fp32 tokens or 2048 of 16 bits a CTA) up to eight such CTAs an SM, above that 4096 tokens
+// a CTA, which leaves two (fp32) or four CTAs an SM at the border; fewer CTAs then scan the history.
+// Measured on rows of 128001, one chunk against 4096 tokens. fp32, no history: 6 rows 5.5 us against
+// 6.5, 9 rows (the last below the border) 6.9 against 7.2, 10 rows 8.0 against 7.5, 16 rows 10.6
+// against 8.7, 48 rows 27 against 20; with 4096 tokens of history 9 rows 14.1 against 11.2, 10
+// rows 15.8 against 11.8. bf16, no history: 10 rows 5.7 against 5.1, 18 rows (the last below) 7.5
+// against 6.9, 20 rows 8.6 against 7.3. One row of 50258 bf16: 3.5 against 4.4.
 template <int kDtype>
 int launch_logits(bd3::LogitParams& p, int64_t B, int sms, void* stream) {
   if (p.S > 1) return launch_logits_u<kDtype, 1, 2>(p, B, sms, stream);

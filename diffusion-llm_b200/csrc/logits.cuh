@@ -23,7 +23,7 @@
 // Measured: 64 x 16 rows of 50258 bf16 logits with bias, mask and histories of 64 to 1024 tokens
 // 50 us (42 us with histories up to 64, where a copy takes 35; the scattered pass over the listed
 // tokens is the rest); 96 fp32 rows of 128001 44 us with histories of up to 16384 (1296 in the
-// mean), 38 with up to 64, 81 with 16384 each: every slice's CTA scans all of its sequence's
+// mean), 40 with 64 each, 84 with 16384 each: every slice's CTA scans all of its sequence's
 // history, from L2. Before, with the counting behind the logits' loads at four CTAs an SM and four
 // rows at a time, those took 53, 46, 55, 40 and 129 us. Slices of 8192 tokens, CTAs of 128, 512 and
 // 1024 threads, eight or more history loads in flight, the next batch loaded ahead (70 against 55),
@@ -97,8 +97,8 @@ __global__ void __launch_bounds__(kLogitThreads, logit_ctas(kDtype, kU, kR))
   using T = LogitTile<kDtype, kU>;
   constexpr int kE = T::kE;
   // Listed tokens are penalised as they stream by: single fp32 rows, whose chunks are four tokens
-  // (96 rows of 128001, histories to 16384: 44 us against 50 by the list; 256 bf16 rows of 32000,
-  // eight tokens a chunk, 16.8 against 14.6).
+  // (96 rows of 128001: histories of 1024 tokens 43 us against 45 by the list, of 16384 84 against
+  // 111; 256 bf16 rows of 32000 with 1024, eight tokens a chunk, 25.6 against 23.4).
   constexpr bool kInline = kR == 1 && kU > 1 && kDtype == 2;
   // The history comes before the loads of the logits, so that its counting has their registers;
   // behind them where a CTA has one chunk a thread and nothing else hides its latency.

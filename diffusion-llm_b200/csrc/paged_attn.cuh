@@ -12,10 +12,12 @@
 // ahead so that no tile waits for a dependent load), and four consumer warps take 16 keys of
 // each tile through mma.sync m16n8k16 (16 rows are far below tcgen05's 64-row minimum, and the
 // tensor cores are nowhere near the bound). Each warp has its own (m, l, O); they are merged in
-// shared memory at the end of the share. Two CTAs an SM keep 160 KB of loads in flight.
+// shared memory at the end of the share. Two CTAs an SM keep 160 KB of loads in flight. (Their ten
+// warps put three on a sub-partition, which caps a thread at 168 registers: enough for 16 rows; at
+// 32 rows ptxas spills 96 bytes a thread.)
 // Measured: 32 sequences of 1K to 16K positions, 12 heads, 16 rows each, 74 us (5.7 TB/s, 0.87 of
-// the copy rate); 64 single tokens of 32 heads over 8 KV heads, 1 to 8192 positions, 23 us
-// (3.4 TB/s: most of its 512 items are short and pay their fixed 2 to 3 us a share); one
+// the copy rate); 64 single tokens of 32 heads over 8 KV heads, 1 to 8192 positions, 24 us
+// (3.3 TB/s: most of its 512 items are short and pay their fixed 2 to 3 us a share); one
 // sequence's 16-token block over 1056 positions 9.6 us, most of it launch, one pass of loads and
 // the merge.
 #pragma once

@@ -37,7 +37,8 @@ constexpr int kPtStages = 3;
 constexpr int kPtThreads = 384;
 constexpr int kPtItemCost = 2;     // an item's fixed cost in key tiles
 // Registers a thread, of the 168 that 384 threads launch with: the softmax holds a row's 128
-// scores (at 168 it spilled), the other four warps need few. 256 x 192 + 128 x 120 = 384 x 168;
+// scores (ptxas reports 238 bytes of spill stores a thread without the split, 84 with it), the
+// other four warps need few. 256 x 192 + 128 x 120 = 384 x 168;
 // the host checks that the kernel has the 168 (more than the launch's own would wait for ever).
 constexpr int kPtRegs = 168, kPtRegsSoftmax = 192, kPtRegsOther = 120;
 static_assert(256 * kPtRegsSoftmax + 128 * kPtRegsOther <= kPtThreads * kPtRegs, "register split");

@@ -10,8 +10,8 @@
 // DRAM-bound: the projection is read once and q, k, v are written once, 16 bytes an access. A
 // CTA takes `tpb` tokens; one thread per token finds its sequence, page and row, then the
 // threads share the (token, head, 8 pairs) units. Measured: 5753 tokens of 32 + 2 x 8 f16 heads
-// 15.5 us (4.8 TB/s, 0.73 of the copy rate), 16384 fp32 tokens of 12 + 2 x 12 heads 51.5 us
-// (5.9 TB/s, 0.91); 1024 tokens of a denoising step 4.6 us, latency.
+// 16.6 us (4.5 TB/s, 0.69 of the copy rate), 16384 fp32 tokens of 12 + 2 x 12 heads 52.3 us
+// (5.8 TB/s, 0.88); 1024 tokens of a denoising step 5.1 us, latency.
 #pragma once
 
 #include "kv_rope.cuh"

@@ -231,8 +231,8 @@ __device__ __forceinline__ PagedCursor paged_chunk(const PagedParams& p, PagedSc
   PagedCursor c;
   c.chunk = (total + workers - 1) / workers;
   // not below half the root of the mean item: a long item cut into hundreds of shares would wait
-  // for the merge of as many partials (8 heads over one KV head of 60004 positions: 69.7 us in
-  // 296 shares)
+  // for the merge of as many partials (8 heads over one KV head of 60004 positions: one token 38
+  // us in 296 shares, 20 so; four tokens 70 and 36; 16 tokens, the large kernel's, 112 and 49)
   const int least = static_cast<int>(0.5f * sqrtf(static_cast<float>(total) / (static_cast<float>(pairs) * p.Hkv)));
   if (c.chunk < least) c.chunk = least;
   if (c.chunk < 1) c.chunk = 1;

@@ -294,7 +294,9 @@ BD3_API int bd3_subs_sample_dev(const void* logits, const int64_t* logit_strides
  * positions [0, min((p / block_size + 1) * block_size, kv_len)) of its sequence (the rule of
  * bd3_decode_attn; block_size 1 is causal, block_size >= kv_len bidirectional). A token that
  * sees none (kv_len below the new tokens' count) gets O = 0 and LSE = -inf. Query heads h share
- * KV head h / (Hq / Hkv). What lies in a page past kv_len is never used (NaN included).
+ * KV head h / (Hq / Hkv). What lies in a page past kv_len is never used (NaN included); a V that is
+ * not finite at a position that a sequence's later new tokens see may also reach its earlier ones,
+ * as 0 times it.
  *   q, o: (total_q, Hq, 64), o in dtype or fp32; lse: optional (total_q, Hq) fp32 contiguous.
  *   max_q: the most new tokens of a sequence (host); 0 says that there are none, and nothing is
  *     launched or written. page_size % 8 == 0.
@@ -340,7 +342,8 @@ BD3_API int bd3_qkv_rope_paged(const void* qkv, int64_t qkv_stride, int64_t T, i
  *   x = logits[b, s, v];  if n > 0: x = (x > 0 ? x / repetition[b] : x * repetition[b])
  *                                       - (frequency[b] * n + presence[b])
  *   x += bias[v];  x = -inf if bit v % 32 of allowed word v / 32 is 0
- * in fp32, rounded once to dtype.
+ * in fp32, rounded once to dtype. One history serves the three penalties; where frequency and
+ * presence are to count the generated tokens only, call it once for each.
  *   logits, out: (B, S, V) in dtype (BD3_BF16, BD3_F16, BD3_F32), vocabulary contiguous; out may
  *     be logits; strides[4] = logits, out (batch, row) in elements.
  *   history: device int64 (int32 with history_is_i32) (B, history_cap), row stride
